@@ -50,6 +50,7 @@ typedef enum { NIB_F32 = 0, NIB_F16 = 1, NIB_BF16 = 2 } nib_dtype;
 #define NIB_DEV_BAD_POSITION 2u /* 1-D RoPE position outside the cos/sin table */
 #define NIB_DEV_BAD_BLOCK 4u    /* block-table entry outside [0, num_blocks) */
 #define NIB_DEV_BAD_INDEX 8u    /* token id / DeepStack row outside its range */
+#define NIB_DEV_NO_PAGE 32u     /* a fork found no free page (16 is NIB_DEV_TIMEOUT below) */
 
 NIB_API int nib_abi_version(void);
 NIB_API const char* nib_last_error(void);
@@ -183,6 +184,81 @@ typedef struct nib_decode_attention_args {
 
 NIB_API int64_t nib_decode_attention_workspace_bytes(const nib_decode_attention_args* args);
 NIB_API int nib_decode_attention(const nib_decode_attention_args* args, void* stream);
+
+/* ------------------------------------------------------------------ shared-prefix decode attention */
+
+/* nib_decode_attention for a batch whose groups share their first tokens: group g is the
+ * requests group_offsets[g] <= b < group_offsets[g + 1] (device int32 [num_groups + 1], not
+ * decreasing, within [0, batch]), and the first prefix_lens[g] tokens of all of them hold the
+ * same keys and values. Those tokens are read through the table of the group's first request
+ * that has as many, once for the group; out[b, h] is what nib_decode_attention gives.
+ * A request that is shorter than its group's prefix, or is in no group, is computed by itself.
+ * A prefix may end inside a block. max_prefix_len and attn.max_context_len (host upper bounds,
+ * 0 = from the table width) only choose how the work is split. attn.variant is not used. dtype
+ * bf16 or f16, head_dim 64 or 128, at most 16 q heads per kv head, block_size a multiple of 16.
+ * attn.workspace: nib_shared_prefix_workspace_bytes() bytes. A decreasing or out-of-range
+ * offset, a negative prefix or a bad context length sets NIB_DEV_BAD_INDEX.
+ * No counterpart in the reference (its prefix cache shares pages, but every request reads
+ * them for itself: nanovllm/layers/attention.py:122-130). */
+typedef struct nib_shared_prefix_args {
+  int32_t struct_size; /* sizeof(nib_shared_prefix_args) */
+  int32_t reserved;
+  nib_decode_attention_args attn;
+  const int32_t* group_offsets;
+  const int32_t* prefix_lens;
+  int64_t num_groups;
+  int64_t max_prefix_len;
+} nib_shared_prefix_args;
+
+NIB_API int64_t nib_shared_prefix_workspace_bytes(const nib_shared_prefix_args* args);
+NIB_API int nib_shared_prefix_decode_attention(const nib_shared_prefix_args* args, void* stream);
+
+/* ------------------------------------------------------------------ sparse decode attention */
+
+/* Key bounds of the chunks (`chunk` consecutive tokens inside a block) that the tokens
+ * [start_lens[b], context_lens[b]) of each request lie in: bounds[block, kv head, chunk, 0, :]
+ * = the smallest, [.., 1, :] = the largest value of each key channel over the chunk's tokens
+ * before context_lens[b]. bounds is [num_blocks, num_kv_heads, block_size / chunk, 2, head_dim]
+ * of the cache's dtype, the last three dims contiguous; other chunks keep their bytes. A NaN
+ * key gives NaN bounds. max_new_tokens (host): the most tokens that a request has between
+ * start_lens and context_lens; more set NIB_DEV_BAD_INDEX and are left out from the chunk after.
+ * Two requests may name the same block where their tokens in it are the same.
+ * No counterpart in the reference. */
+NIB_API int nib_paged_key_bounds(int dtype, const void* key_cache, int64_t cache_block_stride,
+                         int64_t cache_slot_stride, int64_t cache_head_stride, int64_t num_blocks,
+                         int64_t block_size, int64_t num_kv_heads, int64_t head_dim, int64_t chunk,
+                         const int32_t* block_tables, int64_t table_stride,
+                         int64_t max_blocks_per_seq, const int32_t* start_lens,
+                         const int32_t* context_lens, int64_t batch, int64_t max_new_tokens,
+                         void* bounds, int64_t bounds_block_stride, int64_t bounds_head_stride,
+                         unsigned int* status, void* stream);
+
+/* nib_decode_attention over top_chunks chunks of each context, chosen for each (request, kv
+ * head): the first and the last chunk, and those of the others with the largest
+ *   score = sum over the kv head's q heads and the channels of max(q lo, q hi),
+ * an upper bound of the heads' summed scores of any token in the chunk. Scores are summed in
+ * 64 bits; the lower index wins a tie; a NaN or infinite score counts as the largest finite
+ * one, a chunk in a block outside [0, num_blocks) as the smallest. Contexts of at most
+ * top_chunks chunks are attended to whole. selected (int32 [batch, num_kv_heads, top_chunks])
+ * receives the chosen chunk indices in ascending order, -1 behind the last.
+ * attn.max_context_len (host, 0 = from the table width) bounds the contexts: longer ones are
+ * cut there and set NIB_DEV_BAD_INDEX. chunk: a multiple of 16 that divides block_size;
+ * top_chunks >= 2; dtypes and shapes as for nib_shared_prefix_decode_attention.
+ * attn.workspace: nib_sparse_decode_workspace_bytes() bytes.
+ * No counterpart in the reference. */
+typedef struct nib_sparse_decode_args {
+  int32_t struct_size; /* sizeof(nib_sparse_decode_args) */
+  int32_t chunk;
+  int32_t top_chunks;
+  int32_t reserved;
+  nib_decode_attention_args attn;
+  const void* bounds;
+  int64_t bounds_block_stride, bounds_head_stride; /* elements */
+  int32_t* selected;
+} nib_sparse_decode_args;
+
+NIB_API int64_t nib_sparse_decode_workspace_bytes(const nib_sparse_decode_args* args);
+NIB_API int nib_sparse_decode_attention(const nib_sparse_decode_args* args, void* stream);
 
 /* ------------------------------------------------------------------ activation */
 
@@ -332,6 +408,61 @@ NIB_API int nib_paged_gather_varlen_noalloc(int dtype, const void* cache, int64_
                                             int64_t table_stride, const int32_t* seq_lens,
                                             int64_t num_seqs, int64_t max_seq_len, void* out,
                                             unsigned int* status, void* stream);
+
+/* Moving whole blocks (pages). A cache is `planes` arrays of num_blocks blocks of block_bytes
+ * bytes (K and V of each layer), plane p at cache + p * plane_stride_bytes; any dtype. Block
+ * tables are int32 [rows, max_blocks_per_seq] with a row stride; ref_counts (int32
+ * [num_blocks]) says how many rows name a block, 0 = free. Outputs are arrays of their own,
+ * contiguous, and must not overlap the inputs; the cache changes in place.
+ * No counterparts in the reference (its block manager counts references on the host and never
+ * moves a block's contents: nanovllm/engine/block_manager.py:66-229). */
+
+/* block dst_blocks[i] = block src_blocks[i] in every plane, i < n <= 65536. A pair with a -1 is
+ * skipped; so is one whose destination is another pair's source or destination
+ * (NIB_DEV_BAD_INDEX: the result would depend on their order) or that names a block outside
+ * [0, num_blocks) (NIB_DEV_BAD_BLOCK). */
+NIB_API int nib_paged_copy_blocks(void* cache, int64_t planes, int64_t plane_stride_bytes, int64_t num_blocks,
+                          int64_t block_bytes, const int32_t* src_blocks, const int32_t* dst_blocks,
+                          int64_t n, unsigned int* status, void* stream);
+
+/* Row children[i] becomes a copy of the sequence in row parents[i], i < n: it shares the
+ * parent's full blocks (their counts rise by one) and gets a free block of its own (the lowest
+ * free ones, in the order of the forks) for a partly filled last one, of which the filled slots
+ * are copied in every plane. copies (int32 [3, n]) receives source block, fresh block and
+ * slots of each fork (-1, -1, 0: nothing to copy). A child row must be empty (length 0) and
+ * named once; other forks (the later ones of a child named twice) do not take place and set
+ * NIB_DEV_BAD_INDEX, those that find no free block NIB_DEV_NO_PAGE, those whose parent's last
+ * block does not exist NIB_DEV_BAD_BLOCK; -1 as parent or child is skipped.
+ * workspace: nib_paged_fork_workspace_bytes() bytes. */
+NIB_API int64_t nib_paged_fork_workspace_bytes(int64_t rows, int64_t n);
+NIB_API int nib_paged_fork(void* cache, int64_t planes, int64_t plane_stride_bytes, int64_t num_blocks,
+                   int64_t block_bytes, int64_t block_size, const int32_t* block_tables,
+                   int64_t table_stride, int64_t rows, int64_t max_blocks_per_seq,
+                   const int32_t* context_lens, const int32_t* ref_counts, const int32_t* parents,
+                   const int32_t* children, int64_t n, int32_t* tables_out, int32_t* lens_out,
+                   int32_t* refs_out, int32_t* copies, void* workspace, int64_t workspace_bytes,
+                   unsigned int* status, void* stream);
+
+/* The rows free_rows[i], i < n, release their blocks: the counts of the first
+ * ceil(length / block_size) entries fall by one (a row named twice: once), the row becomes -1,
+ * its length 0. A count never falls below 0 (NIB_DEV_BAD_INDEX); -1 in the list is skipped. */
+NIB_API int nib_paged_free(const int32_t* block_tables, int64_t table_stride, int64_t rows,
+                   int64_t max_blocks_per_seq, int64_t block_size, const int32_t* context_lens,
+                   const int32_t* ref_counts, int64_t num_blocks, const int32_t* free_rows, int64_t n,
+                   int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, unsigned int* status,
+                   void* stream);
+
+/* The live blocks (count > 0) move into the first `live` places: the i-th live block behind
+ * them to the i-th free place among them, in ascending order. Table entries and counts follow;
+ * live (int32 [1]) receives their number, moves (int32 [2, num_blocks / 2]) source and
+ * destination of each move, -1 behind the last. The contents of the places that become free
+ * stay as they were. workspace: nib_paged_compact_workspace_bytes() bytes. */
+NIB_API int64_t nib_paged_compact_workspace_bytes(int64_t num_blocks);
+NIB_API int nib_paged_compact(void* cache, int64_t planes, int64_t plane_stride_bytes, int64_t num_blocks,
+                      int64_t block_bytes, const int32_t* block_tables, int64_t table_stride, int64_t rows,
+                      int64_t max_blocks_per_seq, const int32_t* ref_counts, int32_t* tables_out,
+                      int32_t* refs_out, int32_t* live, int32_t* moves, void* workspace,
+                      int64_t workspace_bytes, unsigned int* status, void* stream);
 
 /* ------------------------------------------------------------------ rows */
 

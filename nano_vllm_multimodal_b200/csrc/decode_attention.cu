@@ -460,7 +460,7 @@ static int64_t decode_workspace(const nib_decode_attention_args& a, const Decode
   return pl.splits > 1 ? a.batch * a.num_heads * pl.splits * (a.head_dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
-static const char* decode_check(const nib_decode_attention_args* a) {
+const char* decode_check(const nib_decode_attention_args* a) {
   if (a == nullptr || a->struct_size != static_cast<int32_t>(sizeof(nib_decode_attention_args)))
     return "decode_attention: args struct size mismatch";
   if (a->dtype != NIB_BF16 && a->dtype != NIB_F16) return "decode_attention: dtype must be bf16 or f16";

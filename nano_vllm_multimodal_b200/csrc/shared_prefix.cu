@@ -1,0 +1,110 @@
+// Decode attention of a batch whose groups share their first tokens: the shared part is read
+// and computed once for a group, not once for each of its requests.
+//
+// For a group of n requests whose first P tokens are the same, softmax(q K^T) V splits over
+// the token axis: over [0, P) every (request, head) of a kv head is a row of one product
+// against the same K and V; over [P, len) each request has tokens of its own. Both halves
+// leave partials (max, sum, unnormalised output) that the combine kernel joins.
+//
+// Launches: the prefix (row tiles of 16 rows x kv heads x splits of P), the suffixes
+// (requests x kv heads x splits), the combine.
+#include "decode_mma.cuh"
+
+namespace nib {
+
+struct SharedPrefixPlan {
+  int prefix_splits, suffix_splits;
+  int64_t row_tiles;  // an upper bound: every group's last tile may be ragged
+};
+
+static SharedPrefixPlan shared_prefix_plan(const nib_shared_prefix_args& s) {
+  const nib_decode_attention_args& a = s.attn;
+  SharedPrefixPlan pl{};
+  const int group = a.num_heads / a.num_kv_heads;
+  const int64_t cap = a.max_blocks_per_seq * a.block_size;
+  const int64_t max_len = a.max_context_len > 0 && a.max_context_len < cap ? a.max_context_len : cap;
+  const int64_t max_prefix = s.max_prefix_len > 0 && s.max_prefix_len < max_len ? s.max_prefix_len : max_len;
+  pl.row_tiles = (a.batch * group) / 16 + s.num_groups;
+  const int64_t want = 12LL * sm_count();
+  auto splits = [&](int64_t ctas, int64_t tokens) -> int {
+    int64_t n = ctas < 1 || ctas >= want ? 1 : (want + ctas - 1) / ctas;
+    const int64_t by_len = (tokens + 63) / 64;
+    if (n > by_len) n = by_len;
+    return static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
+  };
+  pl.prefix_splits = splits(pl.row_tiles * a.num_kv_heads, max_prefix);
+  pl.suffix_splits = splits(a.batch * a.num_kv_heads, max_len - max_prefix);
+  return pl;
+}
+
+static int64_t shared_prefix_workspace(const nib_shared_prefix_args& s, const SharedPrefixPlan& pl) {
+  return s.attn.batch * s.attn.num_heads * static_cast<int64_t>(pl.prefix_splits + pl.suffix_splits) *
+         (s.attn.head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+template <typename T, int D>
+static int launch_shared_prefix(const nib_shared_prefix_args& s, const SharedPrefixPlan& pl, cudaStream_t st) {
+  const nib_decode_attention_args& a = s.attn;
+  MmaDecodeParams p = mma_params(a, pl.prefix_splits);
+  p.ws = static_cast<float*>(a.workspace);
+  p.slots = pl.prefix_splits + pl.suffix_splits;
+  p.group_offsets = s.group_offsets;
+  p.prefix_lens = s.prefix_lens;
+  p.num_groups = static_cast<int>(s.num_groups);
+  if (s.num_groups > 0) {
+    const int rc = launch_mma_mode<T, D, kDecodePrefix>(a, p, pl.row_tiles * a.num_kv_heads, st);
+    if (rc != NIB_OK) return rc;
+  }
+  p.splits = pl.suffix_splits;
+  p.slot0 = pl.prefix_splits;
+  const int rc = launch_mma_mode<T, D, kDecodeSuffix>(a, p, a.batch * a.num_kv_heads, st);
+  if (rc != NIB_OK) return rc;
+  launch_k_after(combine_partials_kernel<T, D, kDecodeSuffix>, static_cast<unsigned>(a.batch * a.num_heads), D, 0, st, p);
+  return launch_status("shared_prefix_decode_attention");
+}
+
+static const char* shared_prefix_check(const nib_shared_prefix_args* s) {
+  if (s == nullptr || s->struct_size != static_cast<int32_t>(sizeof(nib_shared_prefix_args)))
+    return "shared_prefix_decode_attention: args struct size mismatch";
+  const char* bad = decode_check(&s->attn);
+  if (bad != nullptr) return bad;
+  if (s->num_groups < 0 || s->num_groups > (1 << 20)) return "shared_prefix_decode_attention: bad group count";
+  return nullptr;
+}
+
+}  // namespace nib
+
+using namespace nib;
+
+extern "C" int64_t nib_shared_prefix_workspace_bytes(const nib_shared_prefix_args* s) {
+  if (shared_prefix_check(s) != nullptr) return -1;
+  return shared_prefix_workspace(*s, shared_prefix_plan(*s));
+}
+
+extern "C" int nib_shared_prefix_decode_attention(const nib_shared_prefix_args* s, void* stream) {
+  const char* bad = shared_prefix_check(s);
+  if (bad != nullptr) {
+    set_error("%s", bad);
+    return NIB_ERR_INVALID;
+  }
+  const nib_decode_attention_args& a = s->attn;
+  if (a.batch == 0) return NIB_OK;
+  NIB_REQUIRE(a.q && a.key_cache && a.value_cache && a.block_tables && a.context_lens && a.out &&
+                  (s->num_groups == 0 || (s->group_offsets && s->prefix_lens)),
+              "shared_prefix_decode_attention: null pointer");
+  const int64_t group = a.num_heads / a.num_kv_heads;
+  NIB_REQUIRE((a.batch * group + s->num_groups) * a.num_kv_heads <= 0x7fffffffLL && a.batch * a.num_heads <= 0x7fffffffLL,
+              "shared_prefix_decode_attention: batch too large");
+  NIB_REQUIRE(a.max_blocks_per_seq * a.block_size < (int64_t{1} << 31),
+              "shared_prefix_decode_attention: block table covers 2^31 tokens or more");
+  NIB_SUPPORT(aligned16(a.q) && a.q_batch_stride % 8 == 0 && a.q_head_stride % 8 == 0,
+              "shared_prefix_decode_attention: q must be 16-byte aligned with strides of multiples of 8 elements");
+  NIB_SUPPORT(decode_mma_eligible(a), "shared_prefix_decode_attention: needs bf16/f16, head_dim 64 or 128, at most 16 q "
+              "heads per kv head, a block size that is a multiple of 16 and 16-byte aligned strides");
+  const SharedPrefixPlan pl = shared_prefix_plan(*s);
+  const int64_t need = shared_prefix_workspace(*s, pl);
+  NIB_REQUIRE(a.workspace && a.workspace_bytes >= need && aligned16(a.workspace),
+              "shared_prefix_decode_attention: workspace of %lld bytes needed", static_cast<long long>(need));
+  const cudaStream_t st = as_stream(stream);
+  return NIB_MMA_CASE(a, T, D, launch_shared_prefix<T, D>(*s, pl, st));
+}

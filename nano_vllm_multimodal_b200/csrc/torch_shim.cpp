@@ -480,6 +480,290 @@ Tensor decode_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_
   return out;
 }
 
+// the fields of a paged decode call; `out` and the workspace are the caller's
+nib_decode_attention_args decode_args(const char* what, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                                      const Tensor& lens, const Tensor& block_tables, double scale,
+                                      int64_t max_context_len, const optional<Tensor>& status) {
+  TORCH_CHECK(q.dim() == 3 && q.stride(2) == 1, what, ": q must be [batch, heads, head_dim]");
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() && k_cache.stride(3) == 1 &&
+                  v_cache.strides() == k_cache.strides(),
+              what, ": caches must be [blocks, block_size, kv_heads, head_dim] of one layout");
+  TORCH_CHECK(q.scalar_type() == k_cache.scalar_type() && v_cache.scalar_type() == q.scalar_type(), what,
+              ": q and caches must share a dtype");
+  TORCH_CHECK(q.size(2) == k_cache.size(3), what, ": head_dim mismatch");
+  TORCH_CHECK(lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == q.size(0) && lens.is_contiguous(), what,
+              ": context_lens must be contiguous int32 [batch]");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.size(0) == q.size(0) &&
+                  (block_tables.size(1) <= 1 || block_tables.stride(1) == 1),
+              what, ": block_tables must be int32 [batch, max_blocks]");
+  TORCH_CHECK(max_context_len >= 0, what, ": max_context_len must be >= 0");
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&k_cache, &v_cache, &lens, &block_tables}) on_device(q, *t, what);
+  nib_decode_attention_args a{};
+  a.struct_size = sizeof(a);
+  a.dtype = code_of(q.scalar_type());
+  a.batch = q.size(0);
+  a.num_heads = static_cast<int32_t>(q.size(1));
+  a.num_kv_heads = static_cast<int32_t>(k_cache.size(2));
+  a.head_dim = static_cast<int32_t>(q.size(2));
+  a.q = q.data_ptr();
+  a.q_batch_stride = q.stride(0);
+  a.q_head_stride = q.stride(1);
+  a.key_cache = k_cache.data_ptr();
+  a.value_cache = v_cache.data_ptr();
+  a.cache_block_stride = k_cache.stride(0);
+  a.cache_slot_stride = k_cache.stride(1);
+  a.cache_head_stride = k_cache.stride(2);
+  a.num_blocks = k_cache.size(0);
+  a.block_size = k_cache.size(1);
+  a.block_tables = block_tables.data_ptr<int32_t>();
+  a.block_table_stride = block_tables.stride(0);
+  a.max_blocks_per_seq = block_tables.size(1);
+  a.context_lens = lens.data_ptr<int32_t>();
+  a.scale = static_cast<float>(scale);
+  a.max_context_len = max_context_len;
+  a.status = status_ptr(status);
+  return a;
+}
+
+// bytes of device memory on q's device; kept by the caching allocator
+Tensor workspace_for(const Tensor& q, int64_t need, const char* what) {
+  TORCH_CHECK(need >= 0, what, ": ", "unsupported configuration");
+  return need > 0 ? at::empty({need}, q.options().dtype(at::kByte)) : Tensor();
+}
+
+Tensor shared_prefix_decode_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                                      const Tensor& context_lens, const Tensor& block_tables,
+                                      const Tensor& group_offsets, const Tensor& prefix_lens, double scale,
+                                      int64_t max_prefix_len, int64_t max_context_len,
+                                      const optional<Tensor>& status) {
+  const char* what = "shared_prefix_decode_attention";
+  nib_shared_prefix_args s{};
+  s.struct_size = sizeof(s);
+  s.attn = decode_args(what, q, k_cache, v_cache, context_lens, block_tables, scale, max_context_len, status);
+  TORCH_CHECK(group_offsets.scalar_type() == at::kInt && group_offsets.dim() == 1 && group_offsets.is_contiguous() &&
+                  prefix_lens.scalar_type() == at::kInt && prefix_lens.dim() == 1 && prefix_lens.is_contiguous() &&
+                  group_offsets.size(0) == prefix_lens.size(0) + 1,
+              what, ": group_offsets and prefix_lens must be contiguous int32 [groups + 1] and [groups]");
+  TORCH_CHECK(max_prefix_len >= 0, what, ": max_prefix_len must be >= 0");
+  on_device(q, group_offsets, what);
+  on_device(q, prefix_lens, what);
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (q.numel() == 0) return out;
+  s.group_offsets = group_offsets.data_ptr<int32_t>();
+  s.prefix_lens = prefix_lens.data_ptr<int32_t>();
+  s.num_groups = prefix_lens.size(0);
+  s.max_prefix_len = max_prefix_len;
+  s.attn.out = out.data_ptr();
+  s.attn.out_batch_stride = out.stride(0);
+  s.attn.out_head_stride = out.stride(1);
+  const int64_t need = nib_shared_prefix_workspace_bytes(&s);
+  if (need < 0) check(nib_shared_prefix_decode_attention(&s, stream_of(q)), "nanoinfer_b200::shared_prefix_decode_attention");
+  Tensor ws = workspace_for(q, need, what);
+  s.attn.workspace = need > 0 ? ws.data_ptr() : nullptr;
+  s.attn.workspace_bytes = need;
+  check(nib_shared_prefix_decode_attention(&s, stream_of(q)), "nanoinfer_b200::shared_prefix_decode_attention");
+  return out;
+}
+
+// bounds [blocks, kv_heads, chunks per block, 2, head_dim] next to a cache
+int64_t bounds_chunk(const Tensor& bounds, const Tensor& k_cache, const char* what) {
+  TORCH_CHECK(bounds.dim() == 5 && bounds.size(0) == k_cache.size(0) && bounds.size(1) == k_cache.size(2) &&
+                  bounds.size(3) == 2 && bounds.size(4) == k_cache.size(3) && bounds.size(2) >= 1 &&
+                  k_cache.size(1) % bounds.size(2) == 0,
+              what, ": bounds must be [blocks, kv_heads, block_size / chunk, 2, head_dim] of the cache");
+  TORCH_CHECK(bounds.scalar_type() == k_cache.scalar_type(), what, ": bounds and cache must share a dtype");
+  TORCH_CHECK(bounds.stride(4) == 1 && bounds.stride(3) == bounds.size(4) && bounds.stride(2) == 2 * bounds.size(4), what,
+              ": the bounds of a block's kv head must be contiguous");
+  on_device(k_cache, bounds, what);
+  return k_cache.size(1) / bounds.size(2);
+}
+
+std::tuple<Tensor, Tensor> sparse_decode_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                                                   const Tensor& bounds, const Tensor& context_lens,
+                                                   const Tensor& block_tables, double scale, int64_t top_chunks,
+                                                   int64_t max_context_len, const optional<Tensor>& status) {
+  const char* what = "sparse_decode_attention";
+  nib_sparse_decode_args s{};
+  s.struct_size = sizeof(s);
+  s.attn = decode_args(what, q, k_cache, v_cache, context_lens, block_tables, scale, max_context_len, status);
+  s.chunk = static_cast<int32_t>(bounds_chunk(bounds, k_cache, what));
+  TORCH_CHECK(top_chunks >= 2 && top_chunks < (int64_t{1} << 31), what, ": top_chunks must be at least 2");
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor selected = at::empty({q.size(0), k_cache.size(2), top_chunks}, q.options().dtype(at::kInt));
+  if (q.numel() == 0) return {out, selected};
+  s.top_chunks = static_cast<int32_t>(top_chunks);
+  s.bounds = bounds.data_ptr();
+  s.bounds_block_stride = bounds.stride(0);
+  s.bounds_head_stride = bounds.stride(1);
+  s.selected = selected.data_ptr<int32_t>();
+  s.attn.out = out.data_ptr();
+  s.attn.out_batch_stride = out.stride(0);
+  s.attn.out_head_stride = out.stride(1);
+  const int64_t need = nib_sparse_decode_workspace_bytes(&s);
+  if (need < 0) check(nib_sparse_decode_attention(&s, stream_of(q)), "nanoinfer_b200::sparse_decode_attention");
+  Tensor ws = workspace_for(q, need, what);
+  s.attn.workspace = need > 0 ? ws.data_ptr() : nullptr;
+  s.attn.workspace_bytes = need;
+  check(nib_sparse_decode_attention(&s, stream_of(q)), "nanoinfer_b200::sparse_decode_attention");
+  return {out, selected};
+}
+
+void paged_key_bounds_(Tensor bounds, const Tensor& k_cache, const Tensor& block_tables, const Tensor& start_lens,
+                       const Tensor& context_lens, int64_t max_new_tokens, const optional<Tensor>& status) {
+  const char* what = "paged_key_bounds_";
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.stride(3) == 1, what, ": cache must be [blocks, block_size, kv_heads, head_dim]");
+  const int64_t chunk = bounds_chunk(bounds, k_cache, what);
+  const int64_t batch = block_tables.size(0);
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 &&
+                  (block_tables.size(1) <= 1 || block_tables.stride(1) == 1),
+              what, ": block_tables must be int32 [batch, max_blocks]");
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&start_lens, &context_lens}) {
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == batch && t->is_contiguous(), what,
+                ": start_lens and context_lens must be contiguous int32 [batch]");
+    on_device(k_cache, *t, what);
+  }
+  TORCH_CHECK(max_new_tokens >= 0, what, ": max_new_tokens must be >= 0");
+  on_device(k_cache, block_tables, what);
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  check(nib_paged_key_bounds(code_of(k_cache.scalar_type()), k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+                             k_cache.stride(2), k_cache.size(0), k_cache.size(1), k_cache.size(2), k_cache.size(3), chunk,
+                             block_tables.data_ptr<int32_t>(), block_tables.stride(0), block_tables.size(1),
+                             start_lens.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(), batch, max_new_tokens,
+                             bounds.data_ptr(), bounds.stride(0), bounds.stride(1), status_ptr(status), stream_of(k_cache)),
+        "nanoinfer_b200::paged_key_bounds_");
+}
+
+// ------------------------------------------------------------------ pages
+
+// a cache as planes of pages: [planes..., blocks, page...] with the page dims contiguous
+struct PageView {
+  void* base;
+  int64_t planes, plane_stride, blocks, block_bytes, first_page_dim;
+};
+
+PageView page_view(const Tensor& cache, int64_t block_dim, const char* what) {
+  const int64_t dims = cache.dim(), bd = block_dim < 0 ? block_dim + dims : block_dim;
+  TORCH_CHECK(bd >= 0 && bd < dims, what, ": block_dim ", block_dim, " of a cache of ", dims, " dims");
+  const int64_t es = static_cast<int64_t>(cache.element_size());
+  PageView v{cache.data_ptr(), 1, 0, cache.size(bd), es, bd + 1};
+  int64_t page = 1;
+  for (int64_t d = dims - 1; d > bd; --d) {
+    TORCH_CHECK(cache.size(d) == 1 || cache.stride(d) == page, what, ": the contents of a block must be contiguous");
+    page *= cache.size(d);
+  }
+  TORCH_CHECK(v.blocks <= 1 || cache.stride(bd) == page, what, ": the blocks must lie one behind the other");
+  int64_t next = 0;  // the stride that the next outer dim must have
+  for (int64_t d = bd - 1; d >= 0; --d) {
+    if (cache.size(d) == 1) continue;
+    TORCH_CHECK(next == 0 || cache.stride(d) == next, what, ": the dims before the blocks must have one stride");
+    if (next == 0) v.plane_stride = cache.stride(d) * es;
+    next = cache.stride(d) * cache.size(d);
+    v.planes *= cache.size(d);
+  }
+  v.block_bytes = page * es;
+  if (cache.numel() == 0) v.planes = 0;
+  if (v.block_bytes == 0) v.block_bytes = es > 1 ? es : 2;  // nothing is moved
+  return v;
+}
+
+void int_list(const Tensor& ref, const Tensor& t, int64_t n, const char* what, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && (n < 0 || t.size(0) == n), what, ": ", name,
+              " must be contiguous int32 [", n < 0 ? std::string("n") : std::to_string(n), "]");
+  on_device(ref, t, what);
+}
+
+void table_rows(const Tensor& ref, const Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), what,
+              ": block_tables must be int32 [rows, max_blocks]");
+  on_device(ref, t, what);
+}
+
+int32_t* ints(const Tensor& t) { return t.numel() ? t.data_ptr<int32_t>() : nullptr; }
+
+void paged_copy_blocks(Tensor cache, const Tensor& src_blocks, const Tensor& dst_blocks, int64_t block_dim,
+                       const optional<Tensor>& status) {
+  const char* what = "paged_copy_blocks";
+  const PageView v = page_view(cache, block_dim, what);
+  int_list(cache, src_blocks, -1, what, "src_blocks");
+  int_list(cache, dst_blocks, src_blocks.size(0), what, "dst_blocks");
+  c10::cuda::CUDAGuard guard(cache.device());
+  check(nib_paged_copy_blocks(v.base, v.planes, v.plane_stride, v.blocks, v.block_bytes, ints(src_blocks), ints(dst_blocks),
+                              src_blocks.size(0), status_ptr(status), stream_of(cache)),
+        "nanoinfer_b200::paged_copy_blocks");
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> paged_fork(Tensor cache, const Tensor& block_tables, const Tensor& context_lens,
+                                                      const Tensor& ref_counts, const Tensor& parents,
+                                                      const Tensor& children, int64_t block_dim,
+                                                      const optional<Tensor>& status) {
+  const char* what = "paged_fork";
+  const PageView v = page_view(cache, block_dim, what);
+  TORCH_CHECK(v.first_page_dim < cache.dim() && cache.size(v.first_page_dim) > 0, what,
+              ": a block's first dim must be its slots");
+  table_rows(cache, block_tables, what);
+  int_list(cache, context_lens, block_tables.size(0), what, "context_lens");
+  int_list(cache, ref_counts, v.blocks, what, "ref_counts");
+  int_list(cache, parents, -1, what, "parents");
+  int_list(cache, children, parents.size(0), what, "children");
+  c10::cuda::CUDAGuard guard(cache.device());
+  const int64_t rows = block_tables.size(0), width = block_tables.size(1), n = parents.size(0);
+  Tensor tables = at::empty({rows, width}, block_tables.options());
+  Tensor lens = at::empty({rows}, block_tables.options());
+  Tensor refs = at::empty({v.blocks}, block_tables.options());
+  Tensor copies = at::empty({3, n}, block_tables.options());
+  const int64_t need = nib_paged_fork_workspace_bytes(rows, n);
+  Tensor ws = workspace_for(cache, need, what);
+  check(nib_paged_fork(v.base, v.planes, v.plane_stride, v.blocks, v.block_bytes, cache.size(v.first_page_dim),
+                       ints(block_tables), block_tables.stride(0), rows, width, ints(context_lens), ints(ref_counts),
+                       ints(parents), ints(children), n, ints(tables), ints(lens), ints(refs), ints(copies),
+                       need > 0 ? ws.data_ptr() : nullptr, need, status_ptr(status), stream_of(cache)),
+        "nanoinfer_b200::paged_fork");
+  return {tables, lens, refs, copies};
+}
+
+std::tuple<Tensor, Tensor, Tensor> paged_free(const Tensor& block_tables, const Tensor& context_lens,
+                                              const Tensor& ref_counts, const Tensor& rows, int64_t block_size,
+                                              const optional<Tensor>& status) {
+  const char* what = "paged_free";
+  table_rows(block_tables, block_tables, what);
+  int_list(block_tables, context_lens, block_tables.size(0), what, "context_lens");
+  int_list(block_tables, ref_counts, -1, what, "ref_counts");
+  int_list(block_tables, rows, -1, what, "rows");
+  TORCH_CHECK(block_size >= 1, what, ": block_size must be positive");
+  c10::cuda::CUDAGuard guard(block_tables.device());
+  Tensor tables = at::empty(block_tables.sizes(), block_tables.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor lens = at::empty(context_lens.sizes(), block_tables.options());
+  Tensor refs = at::empty(ref_counts.sizes(), block_tables.options());
+  check(nib_paged_free(ints(block_tables), block_tables.stride(0), block_tables.size(0), block_tables.size(1), block_size,
+                       ints(context_lens), ints(ref_counts), ref_counts.size(0), ints(rows), rows.size(0), ints(tables),
+                       ints(lens), ints(refs), status_ptr(status), stream_of(block_tables)),
+        "nanoinfer_b200::paged_free");
+  return {tables, lens, refs};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> paged_compact(Tensor cache, const Tensor& block_tables, const Tensor& ref_counts,
+                                                         int64_t block_dim, const optional<Tensor>& status) {
+  const char* what = "paged_compact";
+  const PageView v = page_view(cache, block_dim, what);
+  table_rows(cache, block_tables, what);
+  int_list(cache, ref_counts, v.blocks, what, "ref_counts");
+  c10::cuda::CUDAGuard guard(cache.device());
+  Tensor tables = at::empty(block_tables.sizes(), block_tables.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor refs = at::empty({v.blocks}, block_tables.options());
+  Tensor live = at::empty({1}, block_tables.options());
+  Tensor moves = at::empty({2, v.blocks / 2}, block_tables.options());
+  const int64_t need = nib_paged_compact_workspace_bytes(v.blocks);
+  Tensor ws = workspace_for(cache, need, what);
+  check(nib_paged_compact(v.base, v.planes, v.plane_stride, v.blocks, v.block_bytes, ints(block_tables),
+                          block_tables.stride(0), block_tables.size(0), block_tables.size(1), ints(ref_counts), ints(tables),
+                          ints(refs), live.data_ptr<int32_t>(), ints(moves), ws.data_ptr(), need, status_ptr(status),
+                          stream_of(cache)),
+        "nanoinfer_b200::paged_compact");
+  return {tables, refs, live, moves};
+}
+
 Tensor deepstack_row_index(const Tensor& rows, int64_t tokens, const optional<Tensor>& status) {
   TORCH_CHECK(rows.scalar_type() == at::kLong && rows.dim() == 1, "deepstack_row_index: rows must be int64 [n]");
   TORCH_CHECK(tokens >= 0, "deepstack_row_index: tokens must be >= 0");
@@ -843,6 +1127,21 @@ TORCH_LIBRARY(nanoinfer_b200, m) {
   m.def("deepstack_row_index(Tensor rows, int tokens, Tensor(a!)? status) -> Tensor");
   m.def("decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor context_lens, Tensor block_tables, "
         "float scale, int max_context_len, Tensor(a!)? status, int variant=0) -> Tensor");
+  m.def("shared_prefix_decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor context_lens, "
+        "Tensor block_tables, Tensor group_offsets, Tensor prefix_lens, float scale, int max_prefix_len, "
+        "int max_context_len, Tensor(a!)? status) -> Tensor");
+  m.def("sparse_decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor bounds, Tensor context_lens, "
+        "Tensor block_tables, float scale, int top_chunks, int max_context_len, Tensor(a!)? status) -> (Tensor, Tensor)");
+  m.def("paged_key_bounds_(Tensor(a!) bounds, Tensor k_cache, Tensor block_tables, Tensor start_lens, "
+        "Tensor context_lens, int max_new_tokens, Tensor(b!)? status) -> ()");
+  m.def("paged_copy_blocks(Tensor(a!) cache, Tensor src_blocks, Tensor dst_blocks, int block_dim, "
+        "Tensor(b!)? status) -> ()");
+  m.def("paged_fork(Tensor(a!) cache, Tensor block_tables, Tensor context_lens, Tensor ref_counts, Tensor parents, "
+        "Tensor children, int block_dim, Tensor(b!)? status) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("paged_free(Tensor block_tables, Tensor context_lens, Tensor ref_counts, Tensor rows, int block_size, "
+        "Tensor(a!)? status) -> (Tensor, Tensor, Tensor)");
+  m.def("paged_compact(Tensor(a!) cache, Tensor block_tables, Tensor ref_counts, int block_dim, "
+        "Tensor(b!)? status) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("visual_merge(Tensor tokens, Tensor table, int num_layers, Tensor plan, int num_replacements, "
         "Tensor(a!)? status) -> (Tensor, Tensor)");
   m.def("add_rms_norm_deepstack(Tensor x, Tensor residual, Tensor weight, float eps, Tensor vis, "
@@ -863,6 +1162,13 @@ TORCH_LIBRARY_IMPL(nanoinfer_b200, CUDA, m) {
   m.impl("deepstack_add_", TORCH_FN(nib_torch::deepstack_add_));
   m.impl("deepstack_row_index", TORCH_FN(nib_torch::deepstack_row_index));
   m.impl("decode_attention", TORCH_FN(nib_torch::decode_attention));
+  m.impl("shared_prefix_decode_attention", TORCH_FN(nib_torch::shared_prefix_decode_attention));
+  m.impl("sparse_decode_attention", TORCH_FN(nib_torch::sparse_decode_attention));
+  m.impl("paged_key_bounds_", TORCH_FN(nib_torch::paged_key_bounds_));
+  m.impl("paged_copy_blocks", TORCH_FN(nib_torch::paged_copy_blocks));
+  m.impl("paged_fork", TORCH_FN(nib_torch::paged_fork));
+  m.impl("paged_free", TORCH_FN(nib_torch::paged_free));
+  m.impl("paged_compact", TORCH_FN(nib_torch::paged_compact));
   m.impl("visual_merge", TORCH_FN(nib_torch::visual_merge));
   m.impl("add_rms_norm_deepstack", TORCH_FN(nib_torch::add_rms_norm_deepstack));
 }

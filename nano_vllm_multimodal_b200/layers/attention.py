@@ -166,6 +166,26 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     return ops.decode_attention(q, k_cache, v_cache, context_lens, block_tables, scale, max_context_len)
 
 
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            context_lens: torch.Tensor, block_tables: torch.Tensor, group_offsets: torch.Tensor,
+                            prefix_lens: torch.Tensor, scale: float, max_prefix_len: int = 0,
+                            max_context_len: int = 0) -> torch.Tensor:
+    """:func:`paged_decode_attention` for groups of requests whose first tokens are the same
+    (``ops.shared_prefix_decode_attention``): those tokens are read once for a group."""
+    ints = [t if t.dtype == torch.int32 else t.to(torch.int32)
+            for t in (context_lens, block_tables, group_offsets, prefix_lens)]
+    return ops.shared_prefix_decode_attention(q, k_cache, v_cache, *ints, scale, max_prefix_len, max_context_len)
+
+
+def sparse_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bounds: torch.Tensor,
+                           context_lens: torch.Tensor, block_tables: torch.Tensor, scale: float, top_chunks: int,
+                           max_context_len: int = 0) -> torch.Tensor:
+    """:func:`paged_decode_attention` over the chunks of each context that its key bounds rank
+    highest (``ops.sparse_decode_attention``)."""
+    ints = [t if t.dtype == torch.int32 else t.to(torch.int32) for t in (context_lens, block_tables)]
+    return ops.sparse_decode_attention(q, k_cache, v_cache, bounds, *ints, scale, top_chunks, max_context_len)[0]
+
+
 _FA_DEFAULTS = {"softcap": 0.0, "rotary_interleaved": True, "return_softmax_lse": False}
 
 

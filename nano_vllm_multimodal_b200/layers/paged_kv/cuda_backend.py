@@ -4,7 +4,8 @@ Interface of ``nanovllm/layers/paged_kv/cuda_backend.py:30-104``: allocation
 through the ``torch.classes.nanovllm_paged_kv.PagedKVCache`` owner,
 ``copy_slots_async`` through its pinned transfer stream, and
 ``torch.ops.nanovllm_paged_kv.store/gather`` for the data path. Adds
-``gather_varlen`` (every sequence of a batch in one launch).
+``gather_varlen`` (every sequence of a batch in one launch) and the page
+operators ``copy_blocks``, ``fork``, ``free`` and ``compact``.
 """
 
 from __future__ import annotations
@@ -67,3 +68,27 @@ class CUDAPagedKVBackend:
             raise ValueError("CUDA Paged KV Gather requires CUDA tensors")
         return ops.paged_gather_varlen(cache, block_tables, seq_lens, cu_seqlens, total_tokens,
                                        max_seq_len)
+
+    def copy_blocks(self, cache, src_blocks, dst_blocks, block_dim: int = -4) -> None:
+        """Block ``src_blocks[i]`` to ``dst_blocks[i]`` in every plane of ``[planes..., blocks, ...]``."""
+        if not cache.is_cuda:
+            raise ValueError("CUDA Paged KV page operators require CUDA tensors")
+        ops.paged_copy_blocks(cache, src_blocks, dst_blocks, block_dim)
+
+    def fork(self, cache, block_tables, context_lens, ref_counts, parents, children, block_dim: int = -4):
+        """Sequences that share their parents' full blocks (``ops.paged_fork``)."""
+        if not cache.is_cuda:
+            raise ValueError("CUDA Paged KV page operators require CUDA tensors")
+        return ops.paged_fork(cache, block_tables, context_lens, ref_counts, parents, children, block_dim)
+
+    def free(self, block_tables, context_lens, ref_counts, rows, block_size: int):
+        """Give the blocks of ``rows`` back (``ops.paged_free``)."""
+        if not block_tables.is_cuda:
+            raise ValueError("CUDA Paged KV page operators require CUDA tensors")
+        return ops.paged_free(block_tables, context_lens, ref_counts, rows, block_size)
+
+    def compact(self, cache, block_tables, ref_counts, block_dim: int = -4):
+        """Move the live blocks to the front (``ops.paged_compact``)."""
+        if not cache.is_cuda:
+            raise ValueError("CUDA Paged KV page operators require CUDA tensors")
+        return ops.paged_compact(cache, block_tables, ref_counts, block_dim)

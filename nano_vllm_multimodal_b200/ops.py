@@ -28,6 +28,7 @@ DEV_BAD_SLOT = 1
 DEV_BAD_POSITION = 2
 DEV_BAD_BLOCK = 4
 DEV_BAD_INDEX = 8
+DEV_NO_PAGE = 32
 
 _VALIDATE_ENV = ("NANOINFER_B200_VALIDATE", "NANOVLLM_PAGED_KV_VALIDATE_INDICES")
 _STATUS: dict[int, torch.Tensor] = {}
@@ -72,6 +73,8 @@ def _check_status(st, what: str) -> None:
         names.append("block_table contains an invalid physical block")
     if bits & DEV_BAD_INDEX:
         names.append("an index (token id or row) is out of range")
+    if bits & DEV_NO_PAGE:
+        names.append("no free page is left for a fork")
     raise ValueError(f"{what}: " + "; ".join(names))
 
 
@@ -188,6 +191,61 @@ def paged_gather_varlen(cache, block_tables, seq_lens, cu_seqlens, total_tokens:
     return out
 
 
+# ---------------------------------------------------------------- pages of a cache
+#
+# A cache is ``[planes..., blocks, block_size, kv_heads, head_dim]`` (the runner's allocation is
+# ``[2, layers, blocks, ...]``; one layer's ``[blocks, ...]`` works too); ``block_dim`` names the
+# blocks' dim. Block tables are int32 ``[rows, max_blocks]``, -1 behind a row's last block;
+# ``ref_counts`` (int32 ``[blocks]``) says how many rows name a block, 0: free. The cache changes
+# in place, tables, lengths and counts come back as new tensors.
+
+
+def paged_copy_blocks(cache, src_blocks, dst_blocks, block_dim: int = -4) -> None:
+    """Copy block ``src_blocks[i]`` to ``dst_blocks[i]`` in every plane (``nib_paged_copy_blocks``).
+
+    A pair with a -1 is skipped. A pair whose destination is another pair's source or
+    destination, or that names no block, is left out (validation mode raises)."""
+    st = _status_for(cache)
+    _ops().paged_copy_blocks(cache, src_blocks, dst_blocks, int(block_dim), st)
+    _check_status(st, "paged_copy_blocks")
+
+
+def paged_fork(cache, block_tables, context_lens, ref_counts, parents, children, block_dim: int = -4):
+    """Rows ``children`` become copies of the sequences in rows ``parents`` ->
+    ``(block_tables, context_lens, ref_counts, copies)`` (``nib_paged_fork``).
+
+    A child shares its parent's full blocks and gets the lowest free block for a partly filled
+    last one, whose filled slots are copied; ``copies`` (int32 ``[3, n]``: source block, fresh
+    block, slots; -1 where nothing was copied) moves what a program keeps beside the cache, such
+    as key bounds: ``paged_copy_blocks(bounds, copies[0], copies[1], block_dim=-5)``. Child rows
+    must be empty and distinct; a fork that finds no free block leaves its child empty
+    (validation mode raises)."""
+    st = _status_for(cache)
+    out = _ops().paged_fork(cache, block_tables, context_lens, ref_counts, parents, children, int(block_dim), st)
+    _check_status(st, "paged_fork")
+    return out
+
+
+def paged_free(block_tables, context_lens, ref_counts, rows, block_size: int):
+    """Rows ``rows`` give their blocks back -> ``(block_tables, context_lens, ref_counts)``
+    (``nib_paged_free``): the counts fall by one, the rows become -1 and their lengths 0."""
+    st = _status_for(block_tables)
+    out = _ops().paged_free(block_tables, context_lens, ref_counts, rows, int(block_size), st)
+    _check_status(st, "paged_free")
+    return out
+
+
+def paged_compact(cache, block_tables, ref_counts, block_dim: int = -4):
+    """Move the live blocks to the front -> ``(block_tables, ref_counts, live, moves)``
+    (``nib_paged_compact``): the blocks from ``live`` (int32 ``[1]``) on are free afterwards.
+    ``moves`` (int32 ``[2, blocks // 2]``: source, destination, -1 behind the last) goes to
+    ``paged_copy_blocks`` for what a program keeps beside the cache."""
+    st = _status_for(cache)
+    out = _ops().paged_compact(cache, block_tables, ref_counts, int(block_dim), st)
+    _check_status(st, "paged_compact")
+    return out
+
+
 # ---------------------------------------------------------------- rows
 
 
@@ -242,6 +300,56 @@ def decode_attention(q, k_cache, v_cache, context_lens, block_tables, scale: flo
     out = _ops().decode_attention(q, k_cache, v_cache, context_lens, block_tables, float(scale),
                                   int(max_context_len), st, int(variant))
     _check_status(st, "decode_attention")
+    return out
+
+
+def shared_prefix_decode_attention(q, k_cache, v_cache, context_lens, block_tables, group_offsets, prefix_lens,
+                                   scale: float, max_prefix_len: int = 0, max_context_len: int = 0) -> torch.Tensor:
+    """:func:`decode_attention` for a batch whose groups share their first tokens ->
+    ``[batch, heads, head_dim]`` (``nib_shared_prefix_decode_attention``).
+
+    Group ``g`` is the requests ``group_offsets[g] <= b < group_offsets[g + 1]`` (int32
+    ``[groups + 1]``, not decreasing); the first ``prefix_lens[g]`` tokens of all of them hold the
+    same keys and values (shared pages, or a fork's copies) and are read and computed once for the
+    group. Requests outside the groups, or shorter than their group's prefix, are computed by
+    themselves. ``max_prefix_len`` / ``max_context_len``: optional host upper bounds that only
+    choose how the work is split."""
+    st = _status_for(q)
+    out = _ops().shared_prefix_decode_attention(q, k_cache, v_cache, context_lens, block_tables, group_offsets,
+                                                prefix_lens, float(scale), int(max_prefix_len), int(max_context_len), st)
+    _check_status(st, "shared_prefix_decode_attention")
+    return out
+
+
+def paged_key_bounds_(bounds, k_cache, block_tables, start_lens, context_lens, max_new_tokens: int) -> torch.Tensor:
+    """Refresh, in place, the key bounds of the chunks that tokens ``[start_lens[b],
+    context_lens[b])`` of each request lie in (``nib_paged_key_bounds``).
+
+    ``bounds`` is ``[blocks, kv_heads, block_size // chunk, 2, head_dim]`` of the cache's dtype: the
+    smallest and largest value of each key channel over a chunk's tokens. After a prefill
+    ``start_lens`` are the lengths before it, after a decode step ``context_lens - 1``;
+    ``max_new_tokens`` is a host upper bound of their difference."""
+    st = _status_for(k_cache)
+    _ops().paged_key_bounds_(bounds, k_cache, block_tables, start_lens, context_lens, int(max_new_tokens), st)
+    _check_status(st, "paged_key_bounds_")
+    return bounds
+
+
+def sparse_decode_attention(q, k_cache, v_cache, bounds, context_lens, block_tables, scale: float, top_chunks: int,
+                            max_context_len: int = 0):
+    """Paged decode attention over the ``top_chunks`` chunks of each context with the highest
+    upper bounds of their scores -> ``(out, selected)`` (``nib_sparse_decode_attention``).
+
+    Chosen for each request and kv head: the first and the last chunk always, the others by the
+    sum over the kv head's q heads of the largest ``q . k`` that the chunk's ``bounds`` allow, the
+    lower index first among equals. ``selected`` (int32 ``[batch, kv_heads, top_chunks]``) lists
+    them in ascending order, -1 behind the last. Contexts of at most ``top_chunks`` chunks are
+    attended to whole. ``max_context_len`` (host upper bound, 0: what the tables hold) sizes the
+    workspace; longer contexts are cut there (validation mode raises)."""
+    st = _status_for(q)
+    out = _ops().sparse_decode_attention(q, k_cache, v_cache, bounds, context_lens, block_tables, float(scale),
+                                         int(top_chunks), int(max_context_len), st)
+    _check_status(st, "sparse_decode_attention")
     return out
 
 
