@@ -194,7 +194,8 @@ NIB_API int nib_decode_attention(const nib_decode_attention_args* args, void* st
  * that has as many, once for the group; out[b, h] is what nib_decode_attention gives.
  * A request that is shorter than its group's prefix, or is in no group, is computed by itself.
  * A prefix may end inside a block. max_prefix_len and attn.max_context_len (host upper bounds,
- * 0 = from the table width) only choose how the work is split. attn.variant is not used. dtype
+ * 0 = from the table width) only choose how the work is split. attn.variant: 0 chooses the prefix's
+ * kernel by the rows per group, 1 forces the 16-row kernel, 2 the 256-row one. dtype
  * bf16 or f16, head_dim 64 or 128, at most 16 q heads per kv head, block_size a multiple of 16.
  * attn.workspace: nib_shared_prefix_workspace_bytes() bytes. A decreasing or out-of-range
  * offset, a negative prefix or a bad context length sets NIB_DEV_BAD_INDEX.

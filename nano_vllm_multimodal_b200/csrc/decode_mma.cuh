@@ -588,6 +588,7 @@ combine_partials_kernel(const MmaDecodeParams p) {
   for (int s = s0; s < p.slots; ++s) M = fmaxf(M, ws[s * SW + D]);
   if (M != -INFINITY) {
     for (int s = s0; s < p.slots; ++s) {
+      if (ws[s * SW + D] == -INFINITY) continue;  // a split without tokens
       const float f = ex2_fast(ws[s * SW + D] - M);
       L += ws[s * SW + D + 1] * f;
       A += ws[s * SW + d] * f;
@@ -619,13 +620,15 @@ bool decode_mma_eligible(const nib_decode_attention_args& a);
 const char* decode_check(const nib_decode_attention_args* a);
 size_t decode_mma_smem(int head_dim);
 
-inline int make_cache_map(CUtensorMap* map, const nib_decode_attention_args& a, const void* cache) {
+// boxes of `tokens` consecutive slots of a block x one 64-element half of a head
+inline int make_cache_map(CUtensorMap* map, const nib_decode_attention_args& a, const void* cache,
+                          int tokens = kMmaTile) {
   const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(a.head_dim / 64), static_cast<cuuint64_t>(a.num_kv_heads),
                               static_cast<cuuint64_t>(a.block_size), static_cast<cuuint64_t>(a.num_blocks)};
   const cuuint64_t strides[4] = {128, static_cast<cuuint64_t>(a.cache_head_stride * 2),
                                  static_cast<cuuint64_t>(a.cache_slot_stride * 2),
                                  static_cast<cuuint64_t>(a.cache_block_stride * 2)};
-  const cuuint32_t box[5] = {64, 1, 1, kMmaTile, 1};  // one 64-element half of the head per copy
+  const cuuint32_t box[5] = {64, 1, 1, static_cast<cuuint32_t>(tokens), 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUtensorMapDataType dt =
       a.dtype == NIB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;

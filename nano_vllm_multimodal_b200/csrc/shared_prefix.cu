@@ -12,7 +12,13 @@
 
 namespace nib {
 
+// the prefix kernel of shared_prefix_tc.cu: rows per CTA, tokens per tile, launch
+int64_t prefix_tc_rows();
+int64_t prefix_tc_tile();
+int launch_prefix_tc(const nib_decode_attention_args& a, const MmaDecodeParams& p, int64_t units, cudaStream_t st);
+
 struct SharedPrefixPlan {
+  bool tc;  // the tcgen05 kernel computes the prefixes
   int prefix_splits, suffix_splits;
   int64_t row_tiles;  // an upper bound: every group's last tile may be ragged
 };
@@ -24,7 +30,11 @@ static SharedPrefixPlan shared_prefix_plan(const nib_shared_prefix_args& s) {
   const int64_t cap = a.max_blocks_per_seq * a.block_size;
   const int64_t max_len = a.max_context_len > 0 && a.max_context_len < cap ? a.max_context_len : cap;
   const int64_t max_prefix = s.max_prefix_len > 0 && s.max_prefix_len < max_len ? s.max_prefix_len : max_len;
-  pl.row_tiles = (a.batch * group) / 16 + s.num_groups;
+  // sum over the groups of ceil(rows / tile) <= (all rows + (tile - 1) groups) / tile
+  const int64_t rows = a.batch * group;
+  pl.tc = a.variant == 2 || (a.variant == 0 && rows >= 32 * s.num_groups);
+  const int64_t tile = pl.tc ? prefix_tc_rows() : 16;
+  pl.row_tiles = (rows + (tile - 1) * s.num_groups) / tile;
   const int64_t want = 12LL * sm_count();
   auto splits = [&](int64_t ctas, int64_t tokens) -> int {
     int64_t n = ctas < 1 || ctas >= want ? 1 : (want + ctas - 1) / ctas;
@@ -32,7 +42,22 @@ static SharedPrefixPlan shared_prefix_plan(const nib_shared_prefix_args& s) {
     if (n > by_len) n = by_len;
     return static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
   };
-  pl.prefix_splits = splits(pl.row_tiles * a.num_kv_heads, max_prefix);
+  if (pl.tc) {
+    // one CTA runs on an SM: the split count with the fewest tile steps over all waves, each
+    // CTA's start and end counted as two more
+    const int64_t ctas = pl.row_tiles * a.num_kv_heads, tiles = (max_prefix + prefix_tc_tile() - 1) / prefix_tc_tile();
+    int64_t best = 0;
+    for (int64_t n = 1; n <= tiles && n <= 64; ++n) {
+      const int64_t cost = (ctas * n + sm_count() - 1) / sm_count() * ((tiles + n - 1) / n + 2);
+      if (best == 0 || cost < best) {
+        best = cost;
+        pl.prefix_splits = static_cast<int>(n);
+      }
+    }
+    if (pl.prefix_splits < 1) pl.prefix_splits = 1;
+  } else {
+    pl.prefix_splits = splits(pl.row_tiles * a.num_kv_heads, max_prefix);
+  }
   pl.suffix_splits = splits(a.batch * a.num_kv_heads, max_len - max_prefix);
   return pl;
 }
@@ -52,7 +77,8 @@ static int launch_shared_prefix(const nib_shared_prefix_args& s, const SharedPre
   p.prefix_lens = s.prefix_lens;
   p.num_groups = static_cast<int>(s.num_groups);
   if (s.num_groups > 0) {
-    const int rc = launch_mma_mode<T, D, kDecodePrefix>(a, p, pl.row_tiles * a.num_kv_heads, st);
+    const int rc = pl.tc ? launch_prefix_tc(a, p, pl.row_tiles, st)
+                         : launch_mma_mode<T, D, kDecodePrefix>(a, p, pl.row_tiles * a.num_kv_heads, st);
     if (rc != NIB_OK) return rc;
   }
   p.splits = pl.suffix_splits;
@@ -68,6 +94,7 @@ static const char* shared_prefix_check(const nib_shared_prefix_args* s) {
     return "shared_prefix_decode_attention: args struct size mismatch";
   const char* bad = decode_check(&s->attn);
   if (bad != nullptr) return bad;
+  if (s->attn.variant < 0 || s->attn.variant > 2) return "shared_prefix_decode_attention: bad variant";
   if (s->num_groups < 0 || s->num_groups > (1 << 20)) return "shared_prefix_decode_attention: bad group count";
   return nullptr;
 }

@@ -1,0 +1,453 @@
+// The shared prefix of a group on the 5th-generation tensor cores (tcgen05): every (request,
+// head) of a kv head is a row of one product against the prefix's keys and values.
+//
+// A CTA owns up to 256 rows of a group, a kv head and a split of the prefix's 128-token tiles.
+// Two softmax streams of 128 rows keep the tensor core busy by turns: with more than 128 rows
+// each stream has 128 of them and every tile; else both have the same rows and every other tile,
+// and join their sums at the end. For each of its tiles a stream runs
+//   S = Q K^T      128 x 128 x D, Q and K from shared memory, S in TMEM
+//   P = 2^(S - m)  four warps, a row per thread: no shuffles; P (bf16/f16) over S in TMEM
+//   O += P V       128 x D x 128, P from TMEM, V from shared memory, O in TMEM
+// m is the running maximum, raised only when a tile exceeds it by more than 2^8 (O and the sum
+// are then rescaled): P stays below 2^8 and the fp32 sums cancel the common factor.
+//
+// Warps: 0 loads K and V tiles by TMA (5-D tensor maps over the paged cache, 128-byte swizzle,
+// no multicast) into a ring of five tiles, 1 issues the MMAs, 4-7 and 8-11 are the streams'
+// softmax. Shared memory (224 KB at D = 128) and the 512 TMEM columns (two S, two O) are all of
+// an SM's, so one CTA runs there. K is the K-major B operand; V, whose rows run along d, the
+// MN-major one: no transposition is needed. All waits are bounded; on a timeout the CTA reports
+// NIB_DEV_TIMEOUT, lets its copies land, frees its TMEM and returns.
+#include "decode_mma.cuh"
+#include "tcgen05.cuh"
+
+namespace nib {
+
+constexpr int kPtThreads = 384;
+constexpr int kPtTile = 128;   // tokens per tile
+constexpr int kPtRows = 128;   // rows per stream
+constexpr int kPtSlots = 5;    // ring of K and V tiles
+constexpr float kPtRaise = 8.f;
+
+struct PrefixTcParams {
+  MmaDecodeParams d;
+  int box;  // tokens per TMA copy: the largest power of two that divides block size and tile
+};
+
+template <int D>
+struct PtSmem {
+  static constexpr uint32_t kQ = kPtRows * D * 2;      // one stream's rows
+  static constexpr uint32_t kSlot = kPtTile * D * 2;   // a K or V tile
+  static constexpr uint32_t kBytes = 2 * kQ + kPtSlots * kSlot + 1024;
+};
+
+struct PtBars {
+  uint64_t full[kPtSlots], empty[kPtSlots];
+  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t landed;  // copies of a tile that is mended before it counts as full
+  uint32_t tmem;
+  int abort;
+};
+
+// a bounded wait that also ends when another warp has given up
+__device__ __forceinline__ bool pt_wait(PtBars& s, uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_ns();
+  for (uint32_t it = 0; it < (1u << 30); ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 63u) {
+      if (*reinterpret_cast<volatile int*>(&s.abort)) return false;
+      if (global_ns() - t0 > kWaitLimitNs) break;
+    }
+  }
+  *reinterpret_cast<volatile int*>(&s.abort) = 1;
+  return false;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPtThreads, 1)
+shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                        const PrefixTcParams pp) {
+  using L = PtSmem<D>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int SW = D + 2;
+  __shared__ __align__(8) PtBars bars;
+  extern __shared__ unsigned char dsm_raw[];
+  const MmaDecodeParams& p = pp.d;
+  const uint32_t raw = smem_addr(dsm_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  unsigned char* dsm = dsm_raw + (base - raw);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPtSlots; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 128);
+      mbar_init(&bars.o_done[i], 1);
+    }
+    mbar_init(&bars.landed, 1);
+    bars.abort = 0;
+    fence_mbar_init();
+  }
+  pdl_enter();
+
+  const int kvh = static_cast<int>(blockIdx.x % p.num_kv_heads);
+  const int split = blockIdx.y;
+  const RowTile rt = find_row_tile(p, blockIdx.x / p.num_kv_heads, 2 * kPtRows, lane);
+  if (rt.prefix == 0) return;
+  const int64_t group_rows = (rt.end - rt.first) * p.group;
+  const int rows = static_cast<int>(group_rows - rt.row0 < 2 * kPtRows ? group_rows - rt.row0 : 2 * kPtRows);
+  const bool both = rows > kPtRows;  // each stream has rows of its own
+  const int64_t tiles = (rt.prefix + kPtTile - 1) / kPtTile;
+  const int64_t tile0 = tiles * split / p.splits;
+  const int n = static_cast<int>(tiles * (split + 1) / p.splits - tile0);
+  const int32_t* table = p.tables + rt.leader * p.table_stride;
+  // stream s: its number of tiles and its i-th one; the ring's load number of tile t's K and V
+  // (in the order in which the MMAs want them; a number that has no tile is left out, and no
+  // later one comes round to its slot)
+  auto steps = [&](int s) { return both ? n : (n + 1 - s) / 2; };
+  auto tile_of = [&](int s, int i) { return both ? i : 2 * i + s; };
+  auto k_load = [&](int t) { return both ? 2 * t : t == 0 ? 0 : 2 * t - 1; };
+  auto v_load = [&](int t) { return both ? 2 * t + 1 : 2 * t + 2; };
+
+  // ---- Q rows into shared memory (swizzled 128-byte rows, one 16 KB region per 64 channels)
+  {
+    constexpr int kVecs = D / 8;
+    const bool flip = p.qscale < 0.f;  // the maximum is taken before the scale
+    const int have = both ? 2 * kPtRows : kPtRows;
+    for (int e = threadIdx.x; e < have * kVecs; e += kPtThreads) {
+      const int r = e / kVecs, c = e % kVecs;
+      uint4 v = zero_vec();
+      if (r < rows) {
+        const int64_t row = rt.row0 + r;
+        v = ld_vec(static_cast<const T*>(p.q) + (rt.first + row / p.group) * p.q_bs +
+                   (kvh * p.group + row % p.group) * p.q_hs + c * 8);
+        if (flip) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+      }
+      const int in = r % kPtRows;
+      const uint32_t at = (r / kPtRows) * L::kQ + (c / 8) * (kPtRows * 128) + in * 128 + (((c % 8) ^ (in & 7)) << 4);
+      *reinterpret_cast<uint4*>(dsm + at) = v;
+    }
+    fence_proxy_async();
+  }
+  if (w == 1) tmem_alloc(&bars.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const uint32_t ring = base + 2 * L::kQ;
+
+  if (w == 0) {
+    // ---------------------------------------------------------------- loads
+    const int boxes = kPtTile / pp.box;
+    const uint32_t box_bytes = static_cast<uint32_t>(pp.box) * D * 2;
+    const int loads = n > 0 ? (both ? 2 * n : 2 * n + 1) : 0;
+    uint32_t landed_phase = 0;
+    for (int num = 0; num < loads; ++num) {
+      // which tile this load brings
+      bool is_v;
+      int t;
+      if (both) {
+        is_v = num & 1;
+        t = num >> 1;
+      } else if (num < 2) {
+        is_v = false;
+        t = num;
+      } else {
+        is_v = (num & 1) == 0;
+        t = is_v ? (num - 2) >> 1 : (num + 1) >> 1;
+      }
+      if (t >= n) continue;
+      const int slot = num % kPtSlots;
+      const int64_t tok = (tile0 + t) * kPtTile;
+      const int64_t at = tok + lane * pp.box;
+      int page = -1;
+      if (lane < boxes && at < rt.prefix) {
+        page = __ldg(table + at / p.block_size);
+        if (page < 0 || page >= p.num_blocks) {
+          page = -1;
+          flag(p.status, NIB_DEV_BAD_BLOCK);
+        }
+      }
+      const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+      const bool whole = __popc(have) == boxes && tok + kPtTile <= rt.prefix;
+      bool ok = true;
+      if (num >= kPtSlots) ok = pt_wait(bars, &bars.empty[slot], static_cast<uint32_t>((num / kPtSlots - 1) & 1));
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const bool mend = is_v && !whole;  // rows behind the prefix or without a page become zeros: 0 x NaN is NaN
+      uint64_t* bar = mend ? &bars.landed : &bars.full[slot];
+      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * box_bytes);
+      __syncwarp();
+      if (page >= 0) {
+        const uint32_t dst = ring + slot * L::kSlot + lane * pp.box * 128;
+        const int off = static_cast<int>(at % p.block_size);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_5d(dst + c * (kPtTile * 128), is_v ? &vmap : &kmap, 0, c, kvh, off, page, bar);
+      }
+      if (mend) {
+        ok = pt_wait(bars, &bars.landed, landed_phase);
+        landed_phase ^= 1;
+        if (!__all_sync(0xffffffffu, ok)) break;
+        for (int e = lane; e < kPtTile * (D / 8); e += 32) {
+          const int row = e % kPtTile, c = e / kPtTile;
+          if (tok + row >= rt.prefix || !((have >> (row / pp.box)) & 1u))
+            *reinterpret_cast<uint4*>(dsm + 2 * L::kQ + slot * L::kSlot + (c / 8) * (kPtTile * 128) + row * 128 + (c % 8) * 16) = zero_vec();
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.full[slot]);
+      }
+    }
+  } else if (w == 1) {
+    // ---------------------------------------------------------------- MMAs
+    if (lane == 0) {
+      constexpr uint32_t kIdS = mma_idesc(kBf16, kPtRows, kPtTile, false);
+      constexpr uint32_t kIdO = mma_idesc(kBf16, kPtRows, D, true);
+      auto full = [&](int num) { return pt_wait(bars, &bars.full[num % kPtSlots], static_cast<uint32_t>((num / kPtSlots) & 1)); };
+      auto scores = [&](int s, int i) -> bool {  // S_s = Q_s K^T of the stream's i-th tile
+        const int num = k_load(tile_of(s, i));
+        if (!full(num)) return false;
+        tc_fence_after();
+        const uint32_t q = base + (both ? s * L::kQ : 0u), k = ring + (num % kPtSlots) * L::kSlot;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t at = (kk / 4) * (kPtRows * 128) + (kk % 4) * 32;
+          tc_mma_ss(tmem + s * 128, smem_desc(q + at, 16, 1024), smem_desc(k + at, 16, 1024), kIdS, kk > 0);
+        }
+        tc_commit(&bars.s_full[s]);
+        if (!both || s == 1) tc_commit(&bars.empty[num % kPtSlots]);
+        return true;
+      };
+      bool ok = true;
+      for (int s = 0; s < 2 && ok; ++s)
+        if (steps(s) > 0) ok = scores(s, 0);
+      for (int i = 0; ok && i < steps(0); ++i) {
+        for (int s = 0; s < 2 && ok; ++s) {
+          if (i >= steps(s)) continue;
+          const int num = v_load(tile_of(s, i));
+          ok = pt_wait(bars, &bars.p_full[s], static_cast<uint32_t>(i & 1)) && full(num);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t v = ring + (num % kPtSlots) * L::kSlot;
+#pragma unroll
+          for (int kk = 0; kk < kPtTile / 16; ++kk)
+            tc_mma_ts(tmem + 256 + s * 128, tmem + s * 128 + kk * 8, smem_desc(v + kk * 2048, kPtTile * 128, 1024), kIdO,
+                      i > 0 || kk > 0);
+          tc_commit(&bars.o_done[s]);
+          if (!both || s == 1) tc_commit(&bars.empty[num % kPtSlots]);
+          if (i + 1 < steps(s)) {
+            // the next scores overwrite P: only after the product that reads it
+            ok = pt_wait(bars, &bars.o_done[s], static_cast<uint32_t>(i & 1)) && scores(s, i + 1);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (w >= 4) {
+    // ---------------------------------------------------------------- softmax
+    const int s = (w - 4) >> 2;
+    const uint32_t lanes = static_cast<uint32_t>((w & 3) * 32) << 16;
+    const uint32_t ts = tmem + s * 128 + lanes, to = tmem + 256 + s * 128 + lanes;
+    const float qs = fmaxf(fabsf(p.qscale), 1e-30f);  // masked scores stay -inf with a scale of 0
+    const int mine = steps(s);
+    const int boxes = kPtTile / pp.box;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < mine; ++i) {
+      const int64_t tok = (tile0 + tile_of(s, i)) * kPtTile;
+      const int64_t at = tok + lane * pp.box;
+      bool here = false;
+      if (lane < boxes && at < rt.prefix) {
+        const int page = __ldg(table + at / p.block_size);
+        here = page >= 0 && page < p.num_blocks;
+      }
+      const unsigned have = __ballot_sync(0xffffffffu, here);
+      ok = __all_sync(0xffffffffu, pt_wait(bars, &bars.s_full[s], static_cast<uint32_t>(i & 1)));
+      if (!ok) break;
+      tc_fence_after();
+      // scores behind the prefix or without a page: -inf (warp-uniform, rare)
+      const bool whole = __popc(have) == boxes && tok + kPtTile <= rt.prefix;
+      auto mask = [&](uint32_t* x, int c) {
+        const int64_t left = rt.prefix - tok - c * 32;
+        uint32_t bits = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;  // tokens before the prefix's end
+        if (!((have >> (c * 32 / pp.box)) & 1u)) bits &= 0xffff0000u;
+        if (!((have >> ((c * 32 + 16) / pp.box)) & 1u)) bits &= 0x0000ffffu;
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!((bits >> e) & 1u)) x[e] = 0xff800000u;
+      };
+      // the row is read twice, 32 columns at a time: once for its maximum, once for P
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kPtTile / 32; c += 2) {
+        uint32_t x[64];
+        tmem_ld32(ts + c * 32, x);
+        tmem_ld32(ts + c * 32 + 32, x + 32);
+        tmem_wait_ld();
+        if (!whole) {
+          mask(x, c);
+          mask(x + 32, c + 1);
+        }
+#pragma unroll
+        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(x[e]));
+      }
+      mx *= qs;
+      if (i == 0) {
+        m = mx;
+      } else if (__any_sync(0xffffffffu, mx > m + kPtRaise)) {
+        // raise the maximum of the rows that exceed it; the product before must have ended
+        ok = __all_sync(0xffffffffu, pt_wait(bars, &bars.o_done[s], static_cast<uint32_t>((i - 1) & 1)));
+        if (!ok) break;
+        tc_fence_after();
+        const bool up = mx > m + kPtRaise;
+        const float f = up ? (m == -INFINITY ? 0.f : ex2_fast(m - mx)) : 1.f;
+        m = up ? mx : m;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(to + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st32(to + c * 32, o);
+        }
+      }
+      const float sub = m == -INFINITY ? 0.f : m;  // a row of nothing but masked tokens: all P are 0
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < kPtTile / 32; ++c) {
+        uint32_t x[32], pk[16];
+        tmem_ld32(ts + c * 32, x);
+        tmem_wait_ld();
+        if (!whole) mask(x, c);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float a = ex2_fast(fmaf(__uint_as_float(x[2 * e]), qs, -sub));
+          const float b = ex2_fast(fmaf(__uint_as_float(x[2 * e + 1]), qs, -sub));
+          part[e & 3] += a + b;
+          pk[e] = pack2<T>(a, b);
+        }
+        tmem_st16(ts + c * 16, pk);  // over columns that have been read
+      }
+      l += (part[0] + part[1]) + (part[2] + part[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bars.p_full[s]);
+    }
+    if (ok && mine > 0) ok = __all_sync(0xffffffffu, pt_wait(bars, &bars.o_done[s], static_cast<uint32_t>((mine - 1) & 1)));
+    tc_fence_after();
+    // ---- partials: rows of their own go straight to the workspace; streams of the same rows
+    // meet in shared memory (the ring is free: every tile in it has been used)
+    float* meet = reinterpret_cast<float*>(dsm + 2 * L::kQ);
+    const int r = (w & 3) * 32 + lane;
+    if (!both) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // both streams' last products have ended
+      if (s == 1) {
+        meet[r] = m;
+        meet[kPtRows + r] = l;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(to + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) meet[(2 + c * 32 + e) * kPtRows + r] = mine > 0 ? __uint_as_float(o[e]) : 0.f;
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    const int64_t row = rt.row0 + (both ? s * kPtRows : 0) + r;
+    const bool writes = ok && (both || s == 0) && row < group_rows;
+    float fa = 1.f, fb = 0.f;
+    if (!both && s == 0) {
+      const float m1 = meet[r], top = fmaxf(m, m1);
+      fa = m == -INFINITY ? 0.f : ex2_fast(m - top);
+      fb = m1 == -INFINITY ? 0.f : ex2_fast(m1 - top);
+      l = l * fa + meet[kPtRows + r] * fb;
+      m = top;
+    }
+    if (both || s == 0) {
+      const int64_t b = rt.first + (row < group_rows ? row / p.group : 0);
+      const int h = kvh * p.group + static_cast<int>(row % p.group);
+      float* ws = p.ws + ((b * p.num_heads + h) * p.slots + p.slot0 + split) * SW;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(to + c * 32, o);
+        tmem_wait_ld();
+        if (writes) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float a = mine > 0 ? __uint_as_float(o[e]) : 0.f, bb = mine > 0 ? __uint_as_float(o[e + 1]) : 0.f;
+            if (!both) {
+              a = a * fa + meet[(2 + c * 32 + e) * kPtRows + r] * fb;
+              bb = bb * fa + meet[(3 + c * 32 + e) * kPtRows + r] * fb;
+            }
+            *reinterpret_cast<float2*>(ws + c * 32 + e) = make_float2(a, bb);
+          }
+        }
+      }
+      if (writes) *reinterpret_cast<float2*>(ws + D) = make_float2(m, l);
+    }
+    tc_fence_before();
+  }
+  if (__syncthreads_or(bars.abort) && w == 0) {
+    if (lane == 0) flag(p.status, kDevTimeout);
+    // copies that may still be in flight land before the shared memory goes
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 1000000ull) {
+    }
+  }
+  if (w == 1) {
+    tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+static int tile_box(int64_t block_size) {
+  int box = kPtTile;
+  while (block_size % box != 0) box /= 2;  // at least 16: block sizes are multiples of it
+  return box;
+}
+
+template <typename T, int D>
+static int launch_tc(const nib_decode_attention_args& a, const MmaDecodeParams& d, int64_t units, cudaStream_t st) {
+  PrefixTcParams p{};
+  p.d = d;
+  p.box = tile_box(a.block_size);
+  CUtensorMap kmap, vmap;
+  int rc = make_cache_map(&kmap, a, a.key_cache, p.box);
+  if (rc != NIB_OK) return rc;
+  rc = make_cache_map(&vmap, a, a.value_cache, p.box);
+  if (rc != NIB_OK) return rc;
+  constexpr int smem = static_cast<int>(PtSmem<D>::kBytes);
+  auto kernel = shared_prefix_tc_kernel<T, D>;
+  static int configured[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && configured[dev] < smem) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) {
+      set_error("shared_prefix_decode_attention: cannot reserve shared memory: %s", cudaGetErrorString(e));
+      return NIB_ERR_CUDA;
+    }
+    configured[dev] = smem;
+  }
+  const dim3 grid(static_cast<unsigned>(units * a.num_kv_heads), static_cast<unsigned>(d.splits));
+  launch_k(kernel, grid, kPtThreads, smem, st, kmap, vmap, p);
+  return launch_status("shared_prefix_decode_attention (prefix)");
+}
+
+int64_t prefix_tc_rows() { return 2 * kPtRows; }
+int64_t prefix_tc_tile() { return kPtTile; }
+
+int launch_prefix_tc(const nib_decode_attention_args& a, const MmaDecodeParams& p, int64_t units, cudaStream_t st) {
+  return NIB_MMA_CASE(a, T, D, launch_tc<T, D>(a, p, units, st));
+}
+
+}  // namespace nib

@@ -535,7 +535,7 @@ Tensor shared_prefix_decode_attention(const Tensor& q, const Tensor& k_cache, co
                                       const Tensor& context_lens, const Tensor& block_tables,
                                       const Tensor& group_offsets, const Tensor& prefix_lens, double scale,
                                       int64_t max_prefix_len, int64_t max_context_len,
-                                      const optional<Tensor>& status) {
+                                      const optional<Tensor>& status, int64_t variant) {
   const char* what = "shared_prefix_decode_attention";
   nib_shared_prefix_args s{};
   s.struct_size = sizeof(s);
@@ -554,6 +554,8 @@ Tensor shared_prefix_decode_attention(const Tensor& q, const Tensor& k_cache, co
   s.prefix_lens = prefix_lens.data_ptr<int32_t>();
   s.num_groups = prefix_lens.size(0);
   s.max_prefix_len = max_prefix_len;
+  TORCH_CHECK(variant >= 0 && variant <= 2, what, ": bad variant ", variant);
+  s.attn.variant = static_cast<int32_t>(variant);
   s.attn.out = out.data_ptr();
   s.attn.out_batch_stride = out.stride(0);
   s.attn.out_head_stride = out.stride(1);
@@ -1129,7 +1131,7 @@ TORCH_LIBRARY(nanoinfer_b200, m) {
         "float scale, int max_context_len, Tensor(a!)? status, int variant=0) -> Tensor");
   m.def("shared_prefix_decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor context_lens, "
         "Tensor block_tables, Tensor group_offsets, Tensor prefix_lens, float scale, int max_prefix_len, "
-        "int max_context_len, Tensor(a!)? status) -> Tensor");
+        "int max_context_len, Tensor(a!)? status, int variant=0) -> Tensor");
   m.def("sparse_decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor bounds, Tensor context_lens, "
         "Tensor block_tables, float scale, int top_chunks, int max_context_len, Tensor(a!)? status) -> (Tensor, Tensor)");
   m.def("paged_key_bounds_(Tensor(a!) bounds, Tensor k_cache, Tensor block_tables, Tensor start_lens, "

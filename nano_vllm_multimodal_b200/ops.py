@@ -303,8 +303,12 @@ def decode_attention(q, k_cache, v_cache, context_lens, block_tables, scale: flo
     return out
 
 
+PREFIX_AUTO, PREFIX_ROWS16, PREFIX_ROWS256 = 0, 1, 2
+
+
 def shared_prefix_decode_attention(q, k_cache, v_cache, context_lens, block_tables, group_offsets, prefix_lens,
-                                   scale: float, max_prefix_len: int = 0, max_context_len: int = 0) -> torch.Tensor:
+                                   scale: float, max_prefix_len: int = 0, max_context_len: int = 0,
+                                   variant: int = PREFIX_AUTO) -> torch.Tensor:
     """:func:`decode_attention` for a batch whose groups share their first tokens ->
     ``[batch, heads, head_dim]`` (``nib_shared_prefix_decode_attention``).
 
@@ -313,10 +317,12 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, context_lens, block_tabl
     same keys and values (shared pages, or a fork's copies) and are read and computed once for the
     group. Requests outside the groups, or shorter than their group's prefix, are computed by
     themselves. ``max_prefix_len`` / ``max_context_len``: optional host upper bounds that only
-    choose how the work is split."""
+    choose how the work is split. ``variant`` forces the prefix's kernel: ``PREFIX_ROWS16`` (16 rows
+    a CTA) or ``PREFIX_ROWS256`` (up to 256 rows a CTA, the tcgen05 tensor cores)."""
     st = _status_for(q)
     out = _ops().shared_prefix_decode_attention(q, k_cache, v_cache, context_lens, block_tables, group_offsets,
-                                                prefix_lens, float(scale), int(max_prefix_len), int(max_context_len), st)
+                                                prefix_lens, float(scale), int(max_prefix_len), int(max_context_len), st,
+                                                int(variant))
     _check_status(st, "shared_prefix_decode_attention")
     return out
 

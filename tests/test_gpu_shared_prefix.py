@@ -94,17 +94,21 @@ def test_matches_the_dense_oracle(nq, nkv, dim, dtype, block, groups, alone):
     hinted = _call(c, max_prefix_len=max(1, int(c["prefix"].max())), max_context_len=longest)
     _check(c, hinted, "with bounds")
     assert torch.equal(out, _call(c)), "the same bits twice"
+    for variant in (ops.PREFIX_ROWS16, ops.PREFIX_ROWS256):
+        _check(c, _call(c, variant=variant), f"variant {variant}")
 
 
 def test_long_prefix_and_many_splits():
     c = _case(5, 16, 8, 128, 256, [(20000, [3, 700]), (9001, [1])], [], poison=False)
-    _check(c, _call(c, max_prefix_len=20000, max_context_len=20700))
+    for variant in (ops.PREFIX_ROWS16, ops.PREFIX_ROWS256):
+        _check(c, _call(c, max_prefix_len=20000, max_context_len=20700, variant=variant))
 
 
 @pytest.mark.parametrize("requests", [130, 300])
 def test_many_requests(requests):
     c = _case(requests, 16, 2, 128, 64, [(1500, [i % 50 for i in range(requests)])], [])
-    _check(c, _call(c, max_prefix_len=1500, max_context_len=1550))
+    for variant in (ops.PREFIX_ROWS16, ops.PREFIX_ROWS256):
+        _check(c, _call(c, max_prefix_len=1500, max_context_len=1550, variant=variant))
 
 
 def test_short_and_empty_requests_in_a_group():
@@ -138,7 +142,44 @@ def test_values_of_one_sign_and_extreme_scores():
     e, mean = O.paged_decode_attention(*args).double(), O.paged_decode_attention_abs(*args).double()
     # scores are 30 times the normal ones: their error, 2^-13.7 at 1, is below 30 * 2^-13 each way
     bound = F.attention_bound(c["q"].dtype, e, mean) + 2 * 30 * 2.0 ** -13 * mean
-    assert bool(((_call(c).cpu().double() - e).abs() <= bound).all())
+    for variant in (ops.PREFIX_ROWS16, ops.PREFIX_ROWS256):
+        assert bool(((_call(c, variant=variant).cpu().double() - e).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("variant", [ops.PREFIX_ROWS16, ops.PREFIX_ROWS256])
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+def test_negative_and_zero_scales(variant, scale):
+    c = _case(13, 16, 2, 128, 16, [(200, [5, 40, 3])], [], poison=True)
+    _check(dict(c, scale=scale), _call(dict(c, scale=scale), variant=variant))
+
+
+@pytest.mark.parametrize("variant", [ops.PREFIX_ROWS16, ops.PREFIX_ROWS256])
+def test_rising_maxima_and_bad_prefix_pages(variant):
+    """Keys that grow along the prefix raise every row's maximum tile after tile; a prefix page that
+    does not exist is left out, whatever lies in the memory that its tokens would have come to."""
+    c = _case(14, 16, 1, 128, 32, [(1000, [5, 40, 3, 9, 1, 0, 2, 77, 8, 8])], [], poison=False)
+    c["kc"][c["tables"][0, :31].long()] *= torch.linspace(0.2, 6, 31).to(torch.bfloat16).view(-1, 1, 1, 1)
+    args = (c["q"], c["kc"], c["vc"], c["lens"], c["tables"], c["scale"])
+    e, mean = O.paged_decode_attention(*args).double(), O.paged_decode_attention_abs(*args).double()
+    # scores are up to 6 times the normal ones: their error, 2^-13.7 at 1, is below 6 * 2^-13 each way
+    bound = F.attention_bound(c["q"].dtype, e, mean) + 2 * 6 * 2.0 ** -13 * mean
+    assert bool(((_call(c, variant=variant).cpu().double() - e).abs() <= bound).all())
+    c = _case(15, 16, 8, 128, 16, [(300, [5, 40, 3])], [], poison=True)
+    keep = torch.ones(304, dtype=torch.bool)
+    keep[16 * 7:16 * 8] = False
+    keep[16 * 15:16 * 16] = False
+    c["tables"][0, 7], c["tables"][0, 15] = -1, 10 ** 6  # the first request's table names the prefix
+    out = _call(c, variant=variant)
+    for b in range(3):
+        n = int(c["lens"][b])
+        good = c["tables"][1 if b == 0 else b].clone()  # the shared pages, by a table that has them all
+        row = torch.where((good >= 0) & (torch.arange(len(good)) < 18), good, c["tables"][b])
+        at = torch.tensor([t for t in range(n) if t >= 300 or keep[t]])
+        page = row.long()[at // 16]
+        for h in range(8):
+            e, mean = F.attention(c["q"][b, 2 * h:2 * h + 2], c["kc"][page, at % 16, h], c["vc"][page, at % 16, h], c["scale"])
+            off = (out[b, 2 * h:2 * h + 2].cpu().double() - e).abs()
+            assert bool((off <= F.attention_bound(c["q"].dtype, e, mean)).all()), (b, h)
 
 
 def test_strided_inputs():
