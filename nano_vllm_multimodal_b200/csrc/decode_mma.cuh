@@ -69,9 +69,12 @@ struct MmaDecodeParams {
   float qscale;  // softmax scale * log2(e)
   void* out;
   int64_t o_bs, o_hs;
-  float* ws;  // partials [batch, num_heads, slots, D + 2]; null: one split writes `out`
+  float* ws;   // partials; null: one split writes `out`. kDecodeFull: [batch, num_heads, splits, D + 2]
+               // (output, maximum, sum), else [batch, num_heads, slots, D] with
+  float2* ml;  // [batch, num_heads, slots] (maximum, sum)
   int num_heads, num_kv_heads, group, splits;
   int slots, slot0;  // partials per (request, head), and this launch's first
+  bool early;  // kDecodeSuffix: launched behind the prefix kernel, of whose results it reads none
   unsigned int* status;
   // kDecodeSuffix, kDecodePrefix
   int64_t batch;
@@ -378,7 +381,9 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     fence_mbar_init();
   }
   __syncwarp();
-  pdl_enter();  // the barrier set-up above overlaps the previous kernel's tail
+  // the barrier set-up above overlaps the previous kernel's tail
+  if (MODE == kDecodeSuffix && p.early) pdl_launch_dependents();  // runs next to it; waits for it at the end
+  else pdl_enter();
 
   const int kvh = static_cast<int>(blockIdx.x % p.num_kv_heads);
   const int split = blockIdx.y;
@@ -445,25 +450,63 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
   uint32_t ok_bits = 0;  // per stage: its tile was loaded
   bool timed_out = false;
 
+  // kDecodeFull: a tile's place is looked up when it is issued. Else by 32 tiles of the warp at
+  // once, a tile per lane: the chain list -> table -> copy is too long to walk for each tile.
   const int32_t* list = MODE == kDecodeSparse ? p.selected + (b * p.num_kv_heads + kvh) * p.top : nullptr;
-  // the first token of this warp's tile i; kDecodeSparse: -1 for an entry that names no chunk
-  auto tile_token = [&](int64_t i) -> int64_t {
-    const int64_t t = (tile0 + w + i * kMmaWarps) * kMmaTile;
-    if constexpr (MODE != kDecodeSparse) return t;
-    const int64_t c = __ldg(list + t / p.chunk);
-    return c < 0 || c * p.chunk >= ctx ? -1 : c * p.chunk + t % p.chunk;
-  };
+  int batch_t0 = 0, batch_blk = -1;          // this lane's tile of the batch: first token, block (-1: none)
+  int stage_t0[kMmaStages], stage_ok[kMmaStages];
 
   auto issue = [&](int64_t i) {
     if (i >= n_mine) return;
     const int st = static_cast<int>(i % kMmaStages);
+    if constexpr (MODE != kDecodeFull) {
+      if ((i & 31) == 0) {
+        batch_blk = -1;
+        if (i + lane < n_mine) {
+          int64_t t0 = (tile0 + w + (i + lane) * kMmaWarps) * kMmaTile;
+          if constexpr (MODE == kDecodeSparse) {
+            const int64_t c = __ldg(list + t0 / p.chunk);
+            t0 = c < 0 ? ctx : c * p.chunk + t0 % p.chunk;
+          }
+          batch_t0 = static_cast<int>(t0);
+          if (MODE != kDecodeSparse || t0 < ctx) {  // a last chunk's empty tiles are left out
+            batch_blk = __ldg(table + t0 / p.block_size);
+            if (batch_blk < 0 || batch_blk >= p.num_blocks) {
+              flag(p.status, NIB_DEV_BAD_BLOCK);
+              batch_blk = -1;
+            }
+          }
+        }
+      }
+      const int t0 = __shfl_sync(0xffffffffu, batch_t0, static_cast<int>(i & 31));
+      const int blk = __shfl_sync(0xffffffffu, batch_blk, static_cast<int>(i & 31));
+#pragma unroll
+      for (int s = 0; s < kMmaStages; ++s)
+        if (s == st) {
+          stage_t0[s] = t0;
+          stage_ok[s] = blk >= 0;
+        }
+      if (lane == 0) {
+        fence_proxy_async();  // this stage's generic zero-fill (if any) before the copies
+        mbar_arrive_expect_tx(&bars[w][st], blk >= 0 ? kStageBytes : 0u);
+        if (blk >= 0) {
+          const int off = t0 % p.block_size;
+          const uint32_t dst = ring + st * kStageBytes;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            tma_load_5d(dst + c * kMmaTile * 128, &kmap, 0, c, kvh, off, blk, &bars[w][st]);
+            tma_load_5d(dst + kTileBytes + c * kMmaTile * 128, &vmap, 0, c, kvh, off, blk, &bars[w][st]);
+          }
+        }
+      }
+      return;
+    }
     if (lane == 0) {
-      const int64_t t0 = tile_token(i);
-      const bool named = MODE != kDecodeSparse || (t0 >= 0 && t0 < ctx);  // a last chunk's empty tiles are left out
+      const int64_t t0 = (tile0 + w + i * kMmaWarps) * kMmaTile;
       const int64_t bi = t0 / p.block_size;
-      const int blk = named ? __ldg(table + bi) : -1;
+      const int blk = __ldg(table + bi);
       const bool ok = blk >= 0 && blk < p.num_blocks;
-      if (!ok && named) flag(p.status, NIB_DEV_BAD_BLOCK);
+      if (!ok) flag(p.status, NIB_DEV_BAD_BLOCK);
       fence_proxy_async();  // this stage's generic zero-fill (if any) before the copies
       mbar_arrive_expect_tx(&bars[w][st], ok ? kStageBytes : 0u);
       if (ok) {
@@ -493,8 +536,16 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
       timed_out = true;
       break;
     }
-    const bool ok = (__shfl_sync(0xffffffffu, ok_bits, 0) >> st) & 1u;
-    const int64_t t0 = tile_token(i);
+    bool ok;
+    int64_t t0;
+    if constexpr (MODE == kDecodeFull) {
+      ok = (__shfl_sync(0xffffffffu, ok_bits, 0) >> st) & 1u;
+      t0 = (tile0 + w + i * kMmaWarps) * kMmaTile;
+    } else {
+      ok = st == 0 ? stage_ok[0] : stage_ok[1];
+      t0 = st == 0 ? stage_t0[0] : stage_t0[1];
+      static_assert(kMmaStages == 2, "two stages");
+    }
     const uint32_t kt = ring + st * kStageBytes;
     if (!ok) continue;  // bad block id: its tokens take no part
     // the tile's tokens in [t_begin, t_end), tile-relative (only the first and last tile are partial)
@@ -512,7 +563,10 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     l_a += __shfl_xor_sync(0xffffffffu, l_a, off);
     l_b += __shfl_xor_sync(0xffffffffu, l_b, off);
   }
-  if (__syncthreads_or(timed_out)) return;  // the rows are incomplete; the status bit says so
+  if (__syncthreads_or(timed_out)) {  // the rows are incomplete; the status bit says so
+    if (MODE == kDecodeSuffix && p.early) pdl_wait();
+    return;
+  }
   constexpr int SW = D + 2;
   float* red = reinterpret_cast<float*>(dsm);  // [warps][16 rows][D + 2], over the rings
 #pragma unroll
@@ -556,45 +610,94 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     }
     if (p.ws == nullptr) {
       static_cast<T*>(p.out)[rb * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
-    } else {
-      float* ws = p.ws + ((rb * p.num_heads + h) * p.slots + p.slot0 + split) * SW;
+    } else if constexpr (MODE == kDecodeFull) {
+      float* ws = p.ws + ((rb * p.num_heads + h) * p.splits + split) * SW;
       ws[d] = A;
       if (d == 0) {
         ws[D] = M;
         ws[D + 1] = L;
       }
+    } else {
+      const int64_t at = (rb * p.num_heads + h) * p.slots + p.slot0 + split;
+      p.ws[at * D + d] = A;
+      if (d == 0) p.ml[at] = make_float2(M, L);
     }
   }
+  if (MODE == kDecodeSuffix && p.early) pdl_wait();  // so that the next kernel follows both
 }
 
 
-// out[b, h] from the partials of (b, h). MODE kDecodeSuffix: the first slot0 partials are the
-// prefix's, which only a request that shares one has.
+// out[b, h] from the partials of (b, h): one CTA, its warps by turns over the partials, so that
+// two round trips to memory are all it takes (maxima and sums, then outputs). MODE
+// kDecodeSuffix: the first slot0 partials are the prefix's, which only a request that shares
+// one has.
+constexpr int kCombineWarps = 4;
+
 template <typename T, int D, int MODE>
-__global__ void __launch_bounds__(D)
+__global__ void __launch_bounds__(kCombineWarps * 32)
 combine_partials_kernel(const MmaDecodeParams p) {
   pdl_enter();
-  constexpr int SW = D + 2;
+  constexpr int E = D / 32;  // channels per lane
+  __shared__ float red[kCombineWarps][D];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t bh = blockIdx.x;
   const int64_t b = bh / p.num_heads;
   const int h = static_cast<int>(bh % p.num_heads);
-  const int d = threadIdx.x;
   int s0 = 0;
   if constexpr (MODE == kDecodeSuffix) {
-    if (shared_prefix_of(p, b, clamped_len(p, b, false), d & 31) == 0) s0 = p.slot0;
+    if (shared_prefix_of(p, b, clamped_len(p, b, false), lane) == 0) s0 = p.slot0;
   }
-  const float* ws = p.ws + bh * p.slots * SW;
-  float M = -INFINITY, L = 0.f, A = 0.f;
-  for (int s = s0; s < p.slots; ++s) M = fmaxf(M, ws[s * SW + D]);
+  const float2* ml = p.ml + bh * p.slots;
+  const float* ws = p.ws + bh * p.slots * D + lane * E;
+  float M = -INFINITY;
+  for (int s = s0 + lane; s < p.slots; s += 32) M = fmaxf(M, ml[s].x);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float L = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (M != -INFINITY) {
-    for (int s = s0; s < p.slots; ++s) {
-      if (ws[s * SW + D] == -INFINITY) continue;  // a split without tokens
-      const float f = ex2_fast(ws[s * SW + D] - M);
-      L += ws[s * SW + D + 1] * f;
-      A += ws[s * SW + d] * f;
+    for (int s = s0 + lane; s < p.slots; s += 32) L += ml[s].y * ex2_fast(ml[s].x - M);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+#pragma unroll 4
+    for (int s = s0 + w; s < p.slots; s += kCombineWarps) {
+      const float m = ml[s].x;
+      if (m == -INFINITY) continue;  // a split without tokens: its output is not written
+      const float f = ex2_fast(m - M);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(ws + static_cast<int64_t>(s) * D + e);
+        acc[e] += v.x * f;
+        acc[e + 1] += v.y * f;
+      }
     }
   }
-  static_cast<T*>(p.out)[b * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
+#pragma unroll
+  for (int e = 0; e < E; ++e) red[w][lane * E + e] = acc[e];
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += kCombineWarps * 32) {
+    float A = 0.f;
+#pragma unroll
+    for (int ww = 0; ww < kCombineWarps; ++ww) A += red[ww][d];
+    static_cast<T*>(p.out)[b * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
+  }
+}
+
+// Device bytes of the partials of a launch sequence (any mode but kDecodeFull).
+inline int64_t partial_bytes(const nib_decode_attention_args& a, int64_t slots) {
+  return a.batch * a.num_heads * slots * (a.head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+// their places in `at` (16-byte aligned)
+inline void place_partials(MmaDecodeParams& p, const nib_decode_attention_args& a, void* at) {
+  p.ws = static_cast<float*>(at);
+  p.ml = reinterpret_cast<float2*>(p.ws + a.batch * a.num_heads * static_cast<int64_t>(p.slots) * a.head_dim);
+}
+
+template <typename T, int D, int MODE>
+int launch_combine_partials(const nib_decode_attention_args& a, const MmaDecodeParams& p, cudaStream_t st) {
+  launch_k_after(combine_partials_kernel<T, D, MODE>, static_cast<unsigned>(a.batch * a.num_heads), kCombineWarps * 32, 0, st, p);
+  return launch_status("decode_attention (combine)");
 }
 
 // ------------------------------------------------------------------ host side
@@ -669,8 +772,10 @@ inline MmaDecodeParams mma_params(const nib_decode_attention_args& a, int splits
 }
 
 // The kernel over `row_blocks` (request, kv head) pairs - kDecodePrefix: (row tile, kv head) - and p.splits splits.
+// `after`: behind the kernel before it as a programmatic dependent.
 template <typename T, int D, int MODE>
-int launch_mma_mode(const nib_decode_attention_args& a, const MmaDecodeParams& p, int64_t row_blocks, cudaStream_t st) {
+int launch_mma_mode(const nib_decode_attention_args& a, const MmaDecodeParams& p, int64_t row_blocks, cudaStream_t st,
+                    bool after = false) {
   CUtensorMap kmap, vmap;
   int rc = make_cache_map(&kmap, a, a.key_cache);
   if (rc != NIB_OK) return rc;
@@ -690,7 +795,7 @@ int launch_mma_mode(const nib_decode_attention_args& a, const MmaDecodeParams& p
     configured[dev] = static_cast<int>(smem);
   }
   const dim3 grid(static_cast<unsigned>(row_blocks), static_cast<unsigned>(p.splits));
-  launch_k(kernel, grid, kMmaWarps * 32, smem, st, kmap, vmap, p);
+  launch_k_pdl(after || pdl_enabled(), kernel, grid, kMmaWarps * 32, smem, st, kmap, vmap, p);
   return launch_status("decode_attention (tensor cores)");
 }
 

@@ -509,7 +509,7 @@ extern "C" int nib_paged_fork(void* cache, int64_t planes, int64_t plane_stride_
     m.slots = copies + 2 * n;
     m.max_pairs = n;
     const unsigned grid = move_grid(m, vw, n, n);
-    NIB_VW_SWITCH(vw, VW, launch_k(fork_apply_kernel<VW>, grid, kMoveThreads, 0, st, p, m));
+    NIB_VW_SWITCH(vw, VW, launch_k_after(fork_apply_kernel<VW>, grid, kMoveThreads, 0, st, p, m));
   }
   return launch_status("paged_fork");
 }
@@ -548,7 +548,7 @@ extern "C" int nib_paged_free(const int32_t* block_tables, int64_t table_stride,
   launch_k(free_rows_kernel, static_cast<unsigned>(ctas), kMoveThreads, 0, st, p);
   if (n > 0 && rows > 0) {
     const int64_t row_ctas = rows > 8 * sms ? 8 * sms : rows;
-    launch_k(free_pages_kernel, static_cast<unsigned>(row_ctas), kMoveThreads, 0, st, p);
+    launch_k_after(free_pages_kernel, static_cast<unsigned>(row_ctas), kMoveThreads, 0, st, p);
   }
   return launch_status("paged_free");
 }
@@ -592,6 +592,6 @@ extern "C" int nib_paged_compact(void* cache, int64_t planes, int64_t plane_stri
   launch_k(compact_plan_kernel, 1, kPlanThreads, 0, st, p);
   const int64_t table_ctas = (rows * max_blocks_per_seq + kMoveThreads - 1) / kMoveThreads;
   const unsigned grid = move_grid(m, vw, p.max_moves, table_ctas);
-  NIB_VW_SWITCH(vw, VW, launch_k(compact_apply_kernel<VW>, grid, kMoveThreads, 0, st, p, m));
+  NIB_VW_SWITCH(vw, VW, launch_k_after(compact_apply_kernel<VW>, grid, kMoveThreads, 0, st, p, m));
   return launch_status("paged_compact");
 }

@@ -6,8 +6,10 @@
 // against the same K and V; over [P, len) each request has tokens of its own. Both halves
 // leave partials (max, sum, unnormalised output) that the combine kernel joins.
 //
-// Launches: the prefix (row tiles of 16 rows x kv heads x splits of P), the suffixes
-// (requests x kv heads x splits), the combine.
+// Launches: the prefixes (row tiles x kv heads x splits), the suffixes (requests x kv heads x
+// splits), the combine. The suffix kernel reads nothing of the prefix kernel's: it starts as soon
+// as every CTA of that one has, on SMs that are free and as SMs become free, and waits for it only
+// before its own end, so that the combine follows both.
 #include "decode_mma.cuh"
 
 namespace nib {
@@ -36,9 +38,9 @@ static SharedPrefixPlan shared_prefix_plan(const nib_shared_prefix_args& s) {
   const int64_t tile = pl.tc ? prefix_tc_rows() : 16;
   pl.row_tiles = (rows + (tile - 1) * s.num_groups) / tile;
   const int64_t want = 12LL * sm_count();
-  auto splits = [&](int64_t ctas, int64_t tokens) -> int {
+  auto splits = [&](int64_t ctas, int64_t tokens, int64_t least) -> int {
     int64_t n = ctas < 1 || ctas >= want ? 1 : (want + ctas - 1) / ctas;
-    const int64_t by_len = (tokens + 63) / 64;
+    const int64_t by_len = (tokens + least - 1) / least;
     if (n > by_len) n = by_len;
     return static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
   };
@@ -56,23 +58,22 @@ static SharedPrefixPlan shared_prefix_plan(const nib_shared_prefix_args& s) {
     }
     if (pl.prefix_splits < 1) pl.prefix_splits = 1;
   } else {
-    pl.prefix_splits = splits(pl.row_tiles * a.num_kv_heads, max_prefix);
+    pl.prefix_splits = splits(pl.row_tiles * a.num_kv_heads, max_prefix, 64);
   }
-  pl.suffix_splits = splits(a.batch * a.num_kv_heads, max_len - max_prefix);
+  pl.suffix_splits = splits(a.batch * a.num_kv_heads, max_len - max_prefix, 256);
   return pl;
 }
 
 static int64_t shared_prefix_workspace(const nib_shared_prefix_args& s, const SharedPrefixPlan& pl) {
-  return s.attn.batch * s.attn.num_heads * static_cast<int64_t>(pl.prefix_splits + pl.suffix_splits) *
-         (s.attn.head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  return partial_bytes(s.attn, pl.prefix_splits + pl.suffix_splits);
 }
 
 template <typename T, int D>
 static int launch_shared_prefix(const nib_shared_prefix_args& s, const SharedPrefixPlan& pl, cudaStream_t st) {
   const nib_decode_attention_args& a = s.attn;
   MmaDecodeParams p = mma_params(a, pl.prefix_splits);
-  p.ws = static_cast<float*>(a.workspace);
   p.slots = pl.prefix_splits + pl.suffix_splits;
+  place_partials(p, a, a.workspace);
   p.group_offsets = s.group_offsets;
   p.prefix_lens = s.prefix_lens;
   p.num_groups = static_cast<int>(s.num_groups);
@@ -83,10 +84,10 @@ static int launch_shared_prefix(const nib_shared_prefix_args& s, const SharedPre
   }
   p.splits = pl.suffix_splits;
   p.slot0 = pl.prefix_splits;
-  const int rc = launch_mma_mode<T, D, kDecodeSuffix>(a, p, a.batch * a.num_kv_heads, st);
+  p.early = s.num_groups > 0;
+  const int rc = launch_mma_mode<T, D, kDecodeSuffix>(a, p, a.batch * a.num_kv_heads, st, p.early);
   if (rc != NIB_OK) return rc;
-  launch_k_after(combine_partials_kernel<T, D, kDecodeSuffix>, static_cast<unsigned>(a.batch * a.num_heads), D, 0, st, p);
-  return launch_status("shared_prefix_decode_attention");
+  return launch_combine_partials<T, D, kDecodeSuffix>(a, p, st);
 }
 
 static const char* shared_prefix_check(const nib_shared_prefix_args* s) {

@@ -69,7 +69,6 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                         const PrefixTcParams pp) {
   using L = PtSmem<D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int SW = D + 2;
   __shared__ __align__(8) PtBars bars;
   extern __shared__ unsigned char dsm_raw[];
   const MmaDecodeParams& p = pp.d;
@@ -374,7 +373,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     if (both || s == 0) {
       const int64_t b = rt.first + (row < group_rows ? row / p.group : 0);
       const int h = kvh * p.group + static_cast<int>(row % p.group);
-      float* ws = p.ws + ((b * p.num_heads + h) * p.slots + p.slot0 + split) * SW;
+      const int64_t place = (b * p.num_heads + h) * p.slots + p.slot0 + split;
+      float* ws = p.ws + place * D;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -382,17 +382,18 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         tmem_wait_ld();
         if (writes) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float a = mine > 0 ? __uint_as_float(o[e]) : 0.f, bb = mine > 0 ? __uint_as_float(o[e + 1]) : 0.f;
-            if (!both) {
-              a = a * fa + meet[(2 + c * 32 + e) * kPtRows + r] * fb;
-              bb = bb * fa + meet[(3 + c * 32 + e) * kPtRows + r] * fb;
+          for (int e = 0; e < 32; e += 4) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[k] = mine > 0 ? __uint_as_float(o[e + k]) : 0.f;
+              if (!both) v[k] = v[k] * fa + meet[(2 + c * 32 + e + k) * kPtRows + r] * fb;
             }
-            *reinterpret_cast<float2*>(ws + c * 32 + e) = make_float2(a, bb);
+            *reinterpret_cast<float4*>(ws + c * 32 + e) = make_float4(v[0], v[1], v[2], v[3]);
           }
         }
       }
-      if (writes) *reinterpret_cast<float2*>(ws + D) = make_float2(m, l);
+      if (writes) p.ml[place] = make_float2(m, l);
     }
     tc_fence_before();
   }

@@ -7,8 +7,10 @@
 // (q+ = max(q, 0), q- = min(q, 0)), so over the heads h of a kv head
 //   score(chunk) = a . hi + b . lo,   a = sum_h q_h+,   b = sum_h q_h-
 // bounds the sum of the heads' scores from above with one dot product of 2 D terms, whatever
-// the number of heads. Scores are summed in 64 bits: chunks are ranked by them, and in 32 bits
-// the order of the summation would decide between near neighbours.
+// the number of heads. Chunks are ranked by their scores in 64 bits (in 32, the order of the
+// summation would decide between near neighbours), yet hardly any is computed so: the score
+// kernel sums in 32 bits and bounds its own error, and the selection repeats in 64 bits only the
+// chunks that the bound leaves within reach of the last place - mostly none.
 #include "decode_mma.cuh"
 
 namespace nib {
@@ -41,7 +43,7 @@ constexpr int kBoundsUnroll = 8;
 // One CTA per (window of a request, request): the window's chunk over all kv heads. A thread
 // owns one 16-byte vector of the token row (8 channels of a head) and every slices-th token.
 template <typename T, int D>
-__global__ void __launch_bounds__(kBoundsThreads)
+__global__ void __launch_bounds__(kBoundsThreads, 4)
 key_bounds_kernel(const BoundsParams p) {
   pdl_enter();
   using V2 = typename Vec2<T>::type;
@@ -130,123 +132,184 @@ struct SelectParams {
   MmaDecodeParams d;  // q, tables, lens, heads
   const void* bounds;
   int64_t b_bs, b_hs;
-  uint64_t* keys;      // [batch * kv heads, max_chunks]
+  float2* scores;      // [batch * kv heads, max_chunks]: score in 32 bits, a bound of its error
+  uint64_t* keys;      // as many: the chunks that are scored in 64 bits
   int64_t max_chunks;
   int32_t* selected;   // [batch * kv heads, top]
 };
 
-// A score as a whole number of the same order. -0 counts as 0; NaN and infinity as the largest
-// finite number, so that the first and the last chunk (all ones) rank before every other.
-__device__ __forceinline__ uint64_t score_key(double s) {
-  s = s <= 1.7976931348623157e308 ? s + 0.0 : 1.7976931348623157e308;
-  const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(s));
-  return bits >> 63 ? ~bits : bits | (1ull << 63);
+// A lane's share of a chunk's dot product: 8 channels of lo or of hi. The lanes of a chunk are
+// 2 D / 8, the first half of them lo's.
+template <int D>
+struct ScoreLanes {
+  static constexpr int kLanes = 2 * D / 8;      // per chunk
+  static constexpr int kChunks = 32 / kLanes;   // per warp step
+};
+
+// The lane's eight weights: over the kv head's q heads, the positive parts for hi, the negative
+// ones for lo, summed in 64 bits.
+template <typename T, int D>
+__device__ __forceinline__ void score_weights(const SelectParams& p, int64_t b, int kvh, int lane, double (&wt)[8]) {
+  constexpr int half = ScoreLanes<D>::kLanes / 2;
+  const int part = lane % ScoreLanes<D>::kLanes;
+  const bool is_hi = part >= half;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) wt[i] = 0.0;
+  for (int h = 0; h < p.d.group; ++h) {
+    float f[8];
+    unpack<T>(ld_vec(static_cast<const T*>(p.d.q) + b * p.d.q_bs + (kvh * p.d.group + h) * p.d.q_hs + (part % half) * 8), f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((is_hi ? f[i] > 0.f : f[i] < 0.f) || f[i] != f[i]) wt[i] += static_cast<double>(f[i]);
+  }
+}
+
+// the lane's 16 bytes of chunk c, zeros where its block does not exist
+template <typename T, int D>
+__device__ __forceinline__ uint4 load_bounds(const SelectParams& p, const int32_t* table, int kvh, int64_t c, int lane, bool& ok) {
+  constexpr int half = ScoreLanes<D>::kLanes / 2;
+  const int part = lane % ScoreLanes<D>::kLanes;
+  const int per = p.d.block_size / p.d.chunk;
+  const int blk = __ldg(table + c / per);
+  ok = blk >= 0 && blk < p.d.num_blocks;
+  if (!ok) return zero_vec();
+  return ld_stream(static_cast<const T*>(p.bounds) + blk * p.b_bs + kvh * p.b_hs + ((c % per) * 2 + (part >= half ? 1 : 0)) * D +
+                   (part % half) * 8);
 }
 
 constexpr int kScoreWarps = 8;
-constexpr int kScoreUnroll = 4;
+constexpr int kScoreUnroll = 8;
 
-// A warp takes 32 / (2 D / 8) chunks a step: the lanes of a chunk own 8 channels each, the first
-// half of them of lo, the others of hi.
+// Scores in 32 bits. Error: a weight is rounded once, a lane adds 8 products with fused
+// operations, five shuffles add the lanes: at most 14 roundings of 2^-24 relative to the sum of
+// the terms' absolute values, and that sum (kept next to the score) is itself 2^-20 off at most:
+// 1.25 * 2^-20 of it bounds the error; 2^-126 covers terms too small for relative errors.
+//
+// A warp takes every gridDim.x * kScoreWarps-th group of kScoreUnroll steps of a row (4 KB of
+// bounds) and loads the next group before it works on this one.
 template <typename T, int D>
-__global__ void __launch_bounds__(kScoreWarps * 32)
+__global__ void __launch_bounds__(kScoreWarps * 32, 2)
 chunk_score_kernel(const SelectParams p) {
   pdl_enter();
-  constexpr int LPC = 2 * D / 8;   // lanes per chunk
-  constexpr int CPS = 32 / LPC;    // chunks per warp step
+  constexpr int LPC = ScoreLanes<D>::kLanes, CPS = ScoreLanes<D>::kChunks, G = kScoreUnroll * CPS;
+  constexpr int half = LPC / 2;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t row = blockIdx.y;
   const int64_t b = row / p.d.num_kv_heads;
   const int kvh = static_cast<int>(row % p.d.num_kv_heads);
   const int64_t len = clamped_len(p.d, b, threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0);
-  const int chunk = p.d.chunk;
-  const int64_t chunks = (len + chunk - 1) / chunk;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kScoreWarps * kScoreUnroll * CPS);
-  if (chunks <= p.d.top || first >= chunks) return;  // all of them are selected, or none is here
-  const int part = lane % LPC;
-  const bool is_hi = part >= LPC / 2;
-  const int d0 = (part % (LPC / 2)) * 8;
-  double wt[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) wt[i] = 0.0;
-  for (int h = 0; h < p.d.group; ++h) {
-    float f[8];
-    unpack<T>(ld_vec(static_cast<const T*>(p.d.q) + b * p.d.q_bs + (kvh * p.d.group + h) * p.d.q_hs + d0), f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (is_hi ? f[i] > 0.f : f[i] < 0.f) wt[i] += static_cast<double>(f[i]);
-      else if (f[i] != f[i]) wt[i] += static_cast<double>(f[i]);
-  }
-  const int per = p.d.block_size / chunk;
+  const int chunks = static_cast<int>((len + p.d.chunk - 1) / p.d.chunk);
+  const int step = static_cast<int>(gridDim.x) * kScoreWarps * G;
+  int c0 = (static_cast<int>(blockIdx.x) * kScoreWarps + w) * G;
+  if (chunks <= p.d.top || c0 >= chunks) return;  // all of them are selected, or none is here
   const int32_t* table = p.d.tables + b * p.d.table_stride;
-  const T* base = static_cast<const T*>(p.bounds) + kvh * p.b_hs + (is_hi ? D : 0) + d0;
-  uint4 v[kScoreUnroll];
-  bool ok[kScoreUnroll];
-  const int64_t c0 = first + w * (kScoreUnroll * CPS) + lane / LPC;
+  const int per = p.d.block_size / p.d.chunk;
+  const int part = lane % LPC;
+  const T* base = static_cast<const T*>(p.bounds) + kvh * p.b_hs + (part >= half ? D : 0) + (part % half) * 8;
+  // lane j looks chunk c0 + j of a group up: its block and its place there, -1 for none
+  auto look_up = [&](int c) -> int2 {
+    if (lane >= G || c + lane >= chunks) return make_int2(-1, 0);
+    const int blk = __ldg(table + (c + lane) / per);
+    if (blk >= 0 && blk < p.d.num_blocks) return make_int2(blk, (c + lane) % per);
+    flag(p.d.status, NIB_DEV_BAD_BLOCK);
+    return make_int2(-1, 0);
+  };
+  auto load = [&](int2 place, uint4 (&v)[kScoreUnroll], unsigned& have) {
+    have = __ballot_sync(0xffffffffu, place.x >= 0);
 #pragma unroll
-  for (int j = 0; j < kScoreUnroll; ++j) {
-    const int64_t c = c0 + j * CPS;
-    ok[j] = false;
-    v[j] = zero_vec();
-    if (c < chunks) {
-      const int blk = __ldg(table + c / per);
-      ok[j] = blk >= 0 && blk < p.d.num_blocks;
-      if (ok[j]) v[j] = ld_stream(base + blk * p.b_bs + (c % per) * 2 * D);
-      else flag(p.d.status, NIB_DEV_BAD_BLOCK);
+    for (int j = 0; j < kScoreUnroll; ++j) {
+      const int blk = __shfl_sync(0xffffffffu, place.x, j * CPS + lane / LPC);
+      const int at = __shfl_sync(0xffffffffu, place.y, j * CPS + lane / LPC);
+      v[j] = zero_vec();
+      if (blk >= 0) v[j] = ld_stream(base + blk * p.b_bs + at * 2 * D);
     }
+  };
+  uint4 v[kScoreUnroll];
+  unsigned have;
+  load(look_up(c0), v, have);
+  int2 next_place = look_up(c0 + step);
+  float wt[8];
+  {
+    double exact[8];
+    score_weights<T, D>(p, b, kvh, lane, exact);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wt[i] = static_cast<float>(exact[i]);
   }
+  float2* out = p.scores + row * p.max_chunks;
+  for (; c0 < chunks; c0 += step) {
+    uint4 next[kScoreUnroll];
+    unsigned next_have;
+    load(next_place, next, next_have);
+    next_place = look_up(c0 + 2 * step);
 #pragma unroll
-  for (int j = 0; j < kScoreUnroll; ++j) {
-    const int64_t c = c0 + j * CPS;
-    float f[8];
-    unpack<T>(v[j], f);
-    double s = 0.0;
+    for (int j = 0; j < kScoreUnroll; ++j) {
+      float f[8];
+      unpack<T>(v[j], f);
+      float s = 0.f, a = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = fma(wt[i], static_cast<double>(f[i]), s);
+      for (int i = 0; i < 8; ++i) {
+        s = fmaf(wt[i], f[i], s);
+        a = fmaf(fabsf(wt[i]), fabsf(f[i]), a);
+      }
 #pragma unroll
-    for (int off = LPC / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (part == 0 && c < chunks)
-      p.keys[row * p.max_chunks + c] = c == 0 || c == chunks - 1 ? ~0ull : ok[j] ? score_key(s) : 0ull;
+      for (int off = LPC / 2; off >= 1; off >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, off);
+        a += __shfl_xor_sync(0xffffffffu, a, off);
+      }
+      const int c = c0 + j * CPS + lane / LPC;
+      if (part == 0 && c < chunks) {
+        const float e = fmaf(a, 1.25f * 9.5367431640625e-7f, 1.1754943508222875e-38f);
+        // a chunk without a block ranks below every other (two of them by their index)
+        out[c] = (have >> (j * CPS + lane / LPC)) & 1u ? make_float2(s, e) : make_float2(-INFINITY, 0.f);
+      }
+      v[j] = next[j];
+    }
+    have = next_have;
   }
 }
 
-constexpr int kSelectThreads = 256;
+// A 32-bit score as a whole number of the same order (-0 as 0).
+__device__ __forceinline__ uint32_t key_of(float s) {
+  const uint32_t bits = __float_as_uint(s + 0.f);
+  return bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float score_of(uint32_t key) {
+  return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
 
-// The `top` largest keys of a row, the lower index first among equals, in ascending order of index.
-__global__ void __launch_bounds__(kSelectThreads)
-chunk_select_kernel(const SelectParams p) {
-  pdl_enter();
-  __shared__ unsigned int hist[256];
-  __shared__ uint64_t s_prefix;
-  __shared__ int s_need;
-  __shared__ int warp_sel[kSelectThreads / 32], warp_eq[kSelectThreads / 32];
-  const int64_t row = blockIdx.x;
-  const int64_t len = clamped_len(p.d, row / p.d.num_kv_heads, false);
-  const int64_t n = (len + p.d.chunk - 1) / p.d.chunk;
-  const int top = p.d.top;
-  int32_t* out = p.selected + row * top;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  if (n <= top) {
-    for (int i = tid; i < top; i += kSelectThreads) out[i] = i < n ? i : -1;
-    return;
-  }
-  const uint64_t* keys = p.keys + row * p.max_chunks;
-  if (tid == 0) {
-    s_prefix = 0;
-    s_need = top;
-  }
-  // the top-th largest key, eight bits at a time
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
+// A 64-bit score likewise; NaN and infinity count as the largest finite number.
+__device__ __forceinline__ uint64_t key_of(double s) {
+  s = s <= 1.7976931348623157e308 ? s + 0.0 : 1.7976931348623157e308;
+  const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(s));
+  return bits >> 63 ? ~bits : bits | (1ull << 63);
+}
+
+constexpr int kSelectThreads = 256;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectShared = 8192;  // chunks whose 32-bit keys are kept in shared memory
+
+// The need-th largest of the keys that key(i, k) yields for i < n (false: i takes no part), eight
+// bits at a time; need becomes how many of those equal to it are among the first need. By the
+// whole CTA.
+template <typename K, typename F>
+__device__ __forceinline__ K nth_largest(int64_t n, int& need, unsigned int* hist, K* s_prefix, int* s_need, F key) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  K prefix = 0;
+  for (int shift = 8 * sizeof(K) - 8; shift >= 0; shift -= 8) {
+    hist[tid] = 0;
+    static_assert(kSelectThreads == 256, "a thread per bin");
     __syncthreads();
-    const uint64_t prefix = s_prefix;
-    const int need = s_need;
-    for (int64_t i = tid; i < n; i += kSelectThreads) {
-      const uint64_t k = keys[i];
-      if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+    for (int64_t i0 = 0; i0 < n; i0 += kSelectThreads) {
+      K k = 0;
+      bool part = i0 + tid < n && key(i0 + tid, k);
+      part = part && (shift == 8 * static_cast<int>(sizeof(K)) - 8 || (k >> (shift + 8)) == prefix);
+      // the keys crowd into few bins: one addition for the lanes that share one
+      const int bin = part ? static_cast<int>(k >> shift) & 255 : 256;
+      const unsigned peers = __match_any_sync(0xffffffffu, bin);
+      if (part && lane == __ffs(peers) - 1) atomicAdd(&hist[bin], static_cast<unsigned>(__popc(peers)));
     }
     __syncthreads();
-    if (w == 0) {  // lane l: bins 255 - 8 l down to 248 - 8 l
+    if (tid < 32) {  // lane l: bins 255 - 8 l down to 248 - 8 l
       int mine = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) mine += static_cast<int>(hist[255 - 8 * lane - j]);
@@ -262,8 +325,8 @@ chunk_select_kernel(const SelectParams p) {
         for (int j = 0; j < 8; ++j) {
           const int bin = 255 - 8 * lane - j;
           if (above + static_cast<int>(hist[bin]) >= need) {
-            s_prefix = (prefix << 8) | static_cast<uint64_t>(bin);
-            s_need = need - above;  // still to take among the keys with this prefix
+            *s_prefix = (prefix << 8) | static_cast<K>(bin);
+            *s_need = need - above;
             break;
           }
           above += static_cast<int>(hist[bin]);
@@ -271,36 +334,170 @@ chunk_select_kernel(const SelectParams p) {
       }
     }
     __syncthreads();
+    prefix = *s_prefix;
+    need = *s_need;
   }
-  const uint64_t bar = s_prefix;
-  const int equal = s_need;
+  return prefix;
+}
+
+// op over the CTA's values
+template <typename V, typename F>
+__device__ __forceinline__ V reduce_cta(V v, V* buf, F op) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = buf[0];
+#pragma unroll
+  for (int j = 1; j < kSelectWarps; ++j) v = op(v, buf[j]);
+  return v;
+}
+
+// The `top` best chunks of a row, in ascending order of index. The first and the last chunk are
+// in; `rest` others are wanted. With T the rest-th largest 32-bit score and E the row's largest
+// error bound, a chunk above T + 2 E is in for certain, one below T - 2 E out, and those between
+// compete in 64 bits for the places that are left (unless the places suffice for all of them).
+// A score or bound that is not finite makes E infinite: then every chunk competes.
+template <typename T, int D>
+__global__ void __launch_bounds__(kSelectThreads)
+chunk_select_kernel(const SelectParams p) {
+  pdl_enter();
+  __shared__ uint32_t s_keys[kSelectShared];
+  __shared__ unsigned int hist[256];
+  __shared__ uint64_t s_prefix64;
+  __shared__ uint32_t s_prefix32;
+  __shared__ int s_need;
+  __shared__ float s_worst[kSelectWarps];
+  __shared__ unsigned long long s_counts[kSelectWarps];
+  __shared__ int warp_in[kSelectWarps], warp_eq[kSelectWarps];
+  const int64_t row = blockIdx.x;
+  const int64_t b = row / p.d.num_kv_heads;
+  const int64_t len = clamped_len(p.d, b, false);
+  const int64_t n = (len + p.d.chunk - 1) / p.d.chunk;
+  const int top = p.d.top;
+  int32_t* out = p.selected + row * top;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (n <= top) {
+    for (int i = tid; i < top; i += kSelectThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const float2* scores = p.scores + row * p.max_chunks;
+  uint64_t* keys = p.keys + row * p.max_chunks;
+  const bool shared = n <= kSelectShared;
+  float worst = 0.f;
+  for (int64_t i = tid; i < n; i += kSelectThreads) {
+    const float2 s = scores[i];
+    // a score that is not finite (but for a missing block's) cannot be trusted
+    const bool fine = s.y <= 3.0e38f && (fabsf(s.x) <= 3.0e38f || s.y == 0.f);
+    worst = fmaxf(worst, fine ? s.y : INFINITY);
+    if (shared) s_keys[i] = key_of(s.x);
+  }
+  worst = reduce_cta(worst, s_worst, [](float x, float y) { return fmaxf(x, y); });  // s_keys are written, too
+  auto key32 = [&](int64_t i) { return shared ? s_keys[i] : key_of(scores[i].x); };
+  auto inner = [&](int64_t i) { return i > 0 && i < n - 1; };
+  int rest = top - 2;
+  float high = INFINITY, low = INFINITY;  // rest = 0: none of the inner chunks
+  if (rest > 0) {
+    if (worst < INFINITY) {
+      int need = rest;
+      const float t = score_of(nth_largest<uint32_t>(n, need, hist, &s_prefix32, &s_need, [&](int64_t i, uint32_t& k) {
+        k = key32(i);
+        return inner(i);
+      }));
+      // rounded outwards
+      high = t + 2.f * worst;
+      low = t - 2.f * worst;
+      high += fabsf(high) * 2.4e-7f;
+      low -= fabsf(low) * 2.4e-7f;
+    } else {
+      low = -INFINITY;
+    }
+  }
+  // those certainly in, and those that compete
+  unsigned long long counts = 0;
+  if (rest > 0)
+    for (int64_t i = tid; i < n; i += kSelectThreads)
+      if (inner(i)) {
+        const float s = score_of(key32(i));
+        counts += s > high ? 1ull << 32 : !(s < low) ? 1ull : 0ull;
+      }
+  counts = reduce_cta(counts, s_counts, [](unsigned long long x, unsigned long long y) { return x + y; });
+  const int sure = static_cast<int>(counts >> 32), band = static_cast<int>(counts & 0xffffffffu);
+  const int places = rest - sure;
+  uint64_t bar = 0;     // 64-bit key that a competing chunk has to exceed
+  int equal = band;     // how many of those that reach it are in
+  const bool ranked = band > places;
+  auto competes = [&](int64_t i) {
+    const float s = score_of(key32(i));
+    return rest > 0 && inner(i) && !(s > high) && !(s < low);
+  };
+  if (ranked) {
+    constexpr int LPC = ScoreLanes<D>::kLanes, CPS = ScoreLanes<D>::kChunks;
+    const int kvh = static_cast<int>(row % p.d.num_kv_heads);
+    const int32_t* table = p.d.tables + b * p.d.table_stride;
+    double wt[8];
+    score_weights<T, D>(p, b, kvh, lane, wt);
+    for (int64_t i0 = w * CPS; i0 < n; i0 += kSelectWarps * CPS) {
+      const int64_t i = i0 + lane / LPC;
+      const bool mine = i < n && competes(i);
+      if (!__any_sync(0xffffffffu, mine)) continue;
+      bool ok = false;
+      const uint4 v = mine ? load_bounds<T, D>(p, table, kvh, i, lane, ok) : zero_vec();
+      float f[8];
+      unpack<T>(v, f);
+      double s = 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = fma(wt[j], static_cast<double>(f[j]), s);
+#pragma unroll
+      for (int off = LPC / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+      if (mine && lane % LPC == 0) keys[i] = ok ? key_of(s) : 0ull;
+    }
+    __syncthreads();
+    int need = places;
+    if (need > 0) {
+      bar = nth_largest<uint64_t>(n, need, hist, &s_prefix64, &s_need, [&](int64_t i, uint64_t& k) {
+        if (!competes(i)) return false;
+        k = keys[i];
+        return true;
+      });
+      equal = need;
+    } else {
+      bar = ~0ull;
+      equal = 0;
+    }
+  }
   int done = 0, done_eq = 0;
   for (int64_t i0 = 0; i0 < n; i0 += kSelectThreads) {
     const int64_t i = i0 + tid;
-    const uint64_t k = i < n ? keys[i] : 0;
-    const bool eq = i < n && k == bar;
+    bool sel = i < n && (!inner(i) || (rest > 0 && score_of(key32(i)) > high));
+    bool eq = false;
+    if (i < n && competes(i)) {
+      if (ranked) {
+        const uint64_t k = keys[i];
+        sel = k > bar;
+        eq = k == bar;
+      } else {
+        sel = true;
+      }
+    }
     const unsigned eqs = __ballot_sync(0xffffffffu, eq);
     if (lane == 0) warp_eq[w] = __popc(eqs);
     __syncthreads();
     int before_eq = done_eq + __popc(eqs & ((1u << lane) - 1));
-    int all_eq = 0;
-    for (int j = 0; j < kSelectThreads / 32; ++j) {
+    for (int j = 0; j < kSelectWarps; ++j) {
       if (j < w) before_eq += warp_eq[j];
-      all_eq += warp_eq[j];
+      done_eq += warp_eq[j];
     }
-    const bool sel = (i < n && k > bar) || (eq && before_eq < equal);
+    sel = sel || (eq && before_eq < equal);
     const unsigned sels = __ballot_sync(0xffffffffu, sel);
-    if (lane == 0) warp_sel[w] = __popc(sels);
+    if (lane == 0) warp_in[w] = __popc(sels);
     __syncthreads();
     int before = done + __popc(sels & ((1u << lane) - 1));
-    int all = 0;
-    for (int j = 0; j < kSelectThreads / 32; ++j) {
-      if (j < w) before += warp_sel[j];
-      all += warp_sel[j];
+    for (int j = 0; j < kSelectWarps; ++j) {
+      if (j < w) before += warp_in[j];
+      done += warp_in[j];
     }
     if (sel) out[before] = static_cast<int32_t>(i);
-    done += all;
-    done_eq += all_eq;
   }
 }
 
@@ -326,9 +523,8 @@ static SparsePlan sparse_plan(const nib_sparse_decode_args& s) {
   if (n > by_len) n = by_len;
   if (n > 256) n = 256;
   pl.splits = static_cast<int>(n < 1 ? 1 : n);
-  pl.keys_bytes = pl.max_chunks > s.top_chunks ? (rows * pl.max_chunks * 8 + 15) / 16 * 16 : 0;
-  pl.partial_bytes = pl.splits > 1 ? a.batch * a.num_heads * static_cast<int64_t>(pl.splits) * (a.head_dim + 2) *
-                                         static_cast<int64_t>(sizeof(float)) : 0;
+  pl.keys_bytes = pl.max_chunks > s.top_chunks ? rows * pl.max_chunks * 16 : 0;
+  pl.partial_bytes = pl.splits > 1 ? nib::partial_bytes(a, pl.splits) : 0;
   return pl;
 }
 
@@ -341,24 +537,26 @@ static int launch_sparse(const nib_sparse_decode_args& s, const SparsePlan& pl, 
   sp.d.chunk = s.chunk;
   sp.d.top = s.top_chunks;
   sp.d.selected = s.selected;
-  sp.d.ws = pl.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + pl.keys_bytes) : nullptr;
+  if (pl.splits > 1) place_partials(sp.d, a, static_cast<char*>(a.workspace) + pl.keys_bytes);
   sp.bounds = s.bounds;
   sp.b_bs = s.bounds_block_stride;
   sp.b_hs = s.bounds_head_stride;
-  sp.keys = static_cast<uint64_t*>(a.workspace);
+  const int64_t rows = a.batch * a.num_kv_heads;
+  sp.scores = static_cast<float2*>(a.workspace);
+  sp.keys = reinterpret_cast<uint64_t*>(sp.scores + rows * pl.max_chunks);
   sp.max_chunks = pl.max_chunks;
   sp.selected = s.selected;
-  const int64_t rows = a.batch * a.num_kv_heads;
   if (pl.keys_bytes > 0) {
-    constexpr int kChunks = kScoreWarps * kScoreUnroll * (32 / (2 * D / 8));
-    const dim3 grid(static_cast<unsigned>((pl.max_chunks + kChunks - 1) / kChunks), static_cast<unsigned>(rows));
+    // two CTAs run on an SM: enough of them for two waves, or for all of a row's chunks at once
+    constexpr int kChunks = kScoreWarps * kScoreUnroll * ScoreLanes<D>::kChunks;
+    const int64_t most = (pl.max_chunks + kChunks - 1) / kChunks, want = (4LL * sm_count() + rows - 1) / rows;
+    const dim3 grid(static_cast<unsigned>(most < want ? most : want), static_cast<unsigned>(rows));
     launch_k(chunk_score_kernel<T, D>, grid, kScoreWarps * 32, 0, st, sp);
   }
-  launch_k(chunk_select_kernel, static_cast<unsigned>(rows), kSelectThreads, 0, st, sp);
-  const int rc = launch_mma_mode<T, D, kDecodeSparse>(a, sp.d, rows, st);
+  launch_k_pdl(pl.keys_bytes > 0 || pdl_enabled(), chunk_select_kernel<T, D>, static_cast<unsigned>(rows), kSelectThreads, 0, st, sp);
+  const int rc = launch_mma_mode<T, D, kDecodeSparse>(a, sp.d, rows, st, true);
   if (rc != NIB_OK || pl.splits == 1) return rc;
-  launch_k_after(combine_partials_kernel<T, D, kDecodeSparse>, static_cast<unsigned>(a.batch * a.num_heads), D, 0, st, sp.d);
-  return launch_status("sparse_decode_attention");
+  return launch_combine_partials<T, D, kDecodeSparse>(a, sp.d, st);
 }
 
 static const char* sparse_check(const nib_sparse_decode_args* s) {
