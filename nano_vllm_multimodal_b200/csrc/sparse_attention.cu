@@ -132,9 +132,11 @@ struct SelectParams {
   MmaDecodeParams d;  // q, tables, lens, heads
   const void* bounds;
   int64_t b_bs, b_hs;
-  float2* scores;      // [batch * kv heads, max_chunks]: score in 32 bits, a bound of its error
-  uint64_t* keys;      // as many: the chunks that are scored in 64 bits
+  float* scores;       // [batch * kv heads, max_chunks] in 32 bits
+  float* errors;       // [batch * kv heads, error_slots]: bounds of what they are off, by warp
+  uint64_t* keys;      // as many as scores: the chunks that are scored in 64 bits
   int64_t max_chunks;
+  int error_slots;
   int32_t* selected;   // [batch * kv heads, top]
 };
 
@@ -182,8 +184,9 @@ constexpr int kScoreUnroll = 8;
 
 // Scores in 32 bits. Error: a weight is rounded once, a lane adds 8 products with fused
 // operations, five shuffles add the lanes: at most 14 roundings of 2^-24 relative to the sum of
-// the terms' absolute values, and that sum (kept next to the score) is itself 2^-20 off at most:
-// 1.25 * 2^-20 of it bounds the error; 2^-126 covers terms too small for relative errors.
+// the terms' absolute values. A warp bounds that sum for all of its chunks at once, by the largest
+// |value| of each channel; the bound's own sum is 2^-20 off at most, so 1.25 * 2^-20 of it covers
+// the error, and 2^-126 terms too small for relative errors.
 //
 // A warp takes every gridDim.x * kScoreWarps-th group of kScoreUnroll steps of a row (4 KB of
 // bounds) and loads the next group before it works on this one.
@@ -201,7 +204,12 @@ chunk_score_kernel(const SelectParams p) {
   const int chunks = static_cast<int>((len + p.d.chunk - 1) / p.d.chunk);
   const int step = static_cast<int>(gridDim.x) * kScoreWarps * G;
   int c0 = (static_cast<int>(blockIdx.x) * kScoreWarps + w) * G;
-  if (chunks <= p.d.top || c0 >= chunks) return;  // all of them are selected, or none is here
+  if (chunks <= p.d.top) return;  // all of them are selected
+  float* error = p.errors + row * p.error_slots + blockIdx.x * kScoreWarps + w;
+  if (c0 >= chunks) {
+    if (lane == 0) *error = 0.f;
+    return;
+  }
   const int32_t* table = p.d.tables + b * p.d.table_stride;
   const int per = p.d.block_size / p.d.chunk;
   const int part = lane % LPC;
@@ -235,7 +243,10 @@ chunk_score_kernel(const SelectParams p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) wt[i] = static_cast<float>(exact[i]);
   }
-  float2* out = p.scores + row * p.max_chunks;
+  float* out = p.scores + row * p.max_chunks;
+  float most[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most[i] = 0.f;
   for (; c0 < chunks; c0 += step) {
     uint4 next[kScoreUnroll];
     unsigned next_have;
@@ -245,27 +256,28 @@ chunk_score_kernel(const SelectParams p) {
     for (int j = 0; j < kScoreUnroll; ++j) {
       float f[8];
       unpack<T>(v[j], f);
-      float s = 0.f, a = 0.f;
+      float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         s = fmaf(wt[i], f[i], s);
-        a = fmaf(fabsf(wt[i]), fabsf(f[i]), a);
+        most[i] = fmaxf(most[i], fabsf(f[i]));
       }
 #pragma unroll
-      for (int off = LPC / 2; off >= 1; off >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, off);
-        a += __shfl_xor_sync(0xffffffffu, a, off);
-      }
+      for (int off = LPC / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
       const int c = c0 + j * CPS + lane / LPC;
-      if (part == 0 && c < chunks) {
-        const float e = fmaf(a, 1.25f * 9.5367431640625e-7f, 1.1754943508222875e-38f);
-        // a chunk without a block ranks below every other (two of them by their index)
-        out[c] = (have >> (j * CPS + lane / LPC)) & 1u ? make_float2(s, e) : make_float2(-INFINITY, 0.f);
-      }
+      // a chunk without a block ranks below every other (two of them by their index)
+      if (part == 0 && c < chunks) out[c] = (have >> (j * CPS + lane / LPC)) & 1u ? s : -INFINITY;
       v[j] = next[j];
     }
     have = next_have;
   }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = fmaf(fabsf(wt[i]), most[i], sum);
+#pragma unroll
+  for (int off = LPC / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (CPS == 2) sum = fmaxf(sum, __shfl_xor_sync(0xffffffffu, sum, 16)) + (sum - sum);  // a NaN stays one
+  if (lane == 0) *error = fmaf(sum, 1.25f * 9.5367431640625e-7f, 1.1754943508222875e-38f);
 }
 
 // A 32-bit score as a whole number of the same order (-0 as 0).
@@ -287,26 +299,25 @@ __device__ __forceinline__ uint64_t key_of(double s) {
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectShared = 8192;  // chunks whose 32-bit keys are kept in shared memory
+constexpr int kSelectBand = 256;     // competing chunks that are ranked by comparing each with each
 
 // The need-th largest of the keys that key(i, k) yields for i < n (false: i takes no part), eight
-// bits at a time; need becomes how many of those equal to it are among the first need. By the
-// whole CTA.
+// bits at a time from bit `top_bit` down (above it all keys are those of `prefix`); need becomes
+// how many of those equal to it are among the first need. By the whole CTA.
 template <typename K, typename F>
-__device__ __forceinline__ K nth_largest(int64_t n, int& need, unsigned int* hist, K* s_prefix, int* s_need, F key) {
+__device__ __forceinline__ K nth_largest(int n, int& need, int top_bit, K prefix, unsigned int* hist, K* s_prefix,
+                                         int* s_need, F key) {
+  static_assert(kSelectThreads == 256, "a thread per bin");
   const int tid = threadIdx.x, lane = tid & 31;
-  K prefix = 0;
-  for (int shift = 8 * sizeof(K) - 8; shift >= 0; shift -= 8) {
+  int done = top_bit + 1;  // bits still open
+  while (done > 0) {
+    const int bits = done < 8 ? done : 8, shift = done - bits;
     hist[tid] = 0;
-    static_assert(kSelectThreads == 256, "a thread per bin");
     __syncthreads();
-    for (int64_t i0 = 0; i0 < n; i0 += kSelectThreads) {
+    for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
       K k = 0;
-      bool part = i0 + tid < n && key(i0 + tid, k);
-      part = part && (shift == 8 * static_cast<int>(sizeof(K)) - 8 || (k >> (shift + 8)) == prefix);
-      // the keys crowd into few bins: one addition for the lanes that share one
-      const int bin = part ? static_cast<int>(k >> shift) & 255 : 256;
-      const unsigned peers = __match_any_sync(0xffffffffu, bin);
-      if (part && lane == __ffs(peers) - 1) atomicAdd(&hist[bin], static_cast<unsigned>(__popc(peers)));
+      if (i0 + tid < n && key(i0 + tid, k) && (k >> (shift + bits - 1)) >> 1 == prefix)
+        atomicAdd(&hist[static_cast<int>(k >> shift) & ((1 << bits) - 1)], 1u);
     }
     __syncthreads();
     if (tid < 32) {  // lane l: bins 255 - 8 l down to 248 - 8 l
@@ -325,7 +336,7 @@ __device__ __forceinline__ K nth_largest(int64_t n, int& need, unsigned int* his
         for (int j = 0; j < 8; ++j) {
           const int bin = 255 - 8 * lane - j;
           if (above + static_cast<int>(hist[bin]) >= need) {
-            *s_prefix = (prefix << 8) | static_cast<K>(bin);
+            *s_prefix = (prefix << bits) | static_cast<K>(bin);
             *s_need = need - above;
             break;
           }
@@ -336,21 +347,9 @@ __device__ __forceinline__ K nth_largest(int64_t n, int& need, unsigned int* his
     __syncthreads();
     prefix = *s_prefix;
     need = *s_need;
+    done = shift;
   }
   return prefix;
-}
-
-// op over the CTA's values
-template <typename V, typename F>
-__device__ __forceinline__ V reduce_cta(V v, V* buf, F op) {
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = buf[0];
-#pragma unroll
-  for (int j = 1; j < kSelectWarps; ++j) v = op(v, buf[j]);
-  return v;
 }
 
 // The `top` best chunks of a row, in ascending order of index. The first and the last chunk are
@@ -364,16 +363,17 @@ chunk_select_kernel(const SelectParams p) {
   pdl_enter();
   __shared__ uint32_t s_keys[kSelectShared];
   __shared__ unsigned int hist[256];
-  __shared__ uint64_t s_prefix64;
+  __shared__ uint64_t s_prefix64, band_key[kSelectBand];
   __shared__ uint32_t s_prefix32;
-  __shared__ int s_need;
-  __shared__ float s_worst[kSelectWarps];
+  __shared__ int s_need, s_band, band_at[kSelectBand];
+  __shared__ bool band_in[kSelectBand];
+  __shared__ uint4 s_range[kSelectWarps];
   __shared__ unsigned long long s_counts[kSelectWarps];
   __shared__ int warp_in[kSelectWarps], warp_eq[kSelectWarps];
   const int64_t row = blockIdx.x;
   const int64_t b = row / p.d.num_kv_heads;
   const int64_t len = clamped_len(p.d, b, false);
-  const int64_t n = (len + p.d.chunk - 1) / p.d.chunk;
+  const int n = static_cast<int>((len + p.d.chunk - 1) / p.d.chunk);
   const int top = p.d.top;
   int32_t* out = p.selected + row * top;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -381,26 +381,51 @@ chunk_select_kernel(const SelectParams p) {
     for (int i = tid; i < top; i += kSelectThreads) out[i] = i < n ? i : -1;
     return;
   }
-  const float2* scores = p.scores + row * p.max_chunks;
-  uint64_t* keys = p.keys + row * p.max_chunks;
+  const float* scores = p.scores + row * p.max_chunks;
   const bool shared = n <= kSelectShared;
+  auto inner = [&](int i) { return i > 0 && i < n - 1; };
+  // the row's error bound (infinite if a score or a bound is not to be trusted: NaN, overflow) and
+  // the range of its inner keys
+  bool fine = true;
   float worst = 0.f;
-  for (int64_t i = tid; i < n; i += kSelectThreads) {
-    const float2 s = scores[i];
-    // a score that is not finite (but for a missing block's) cannot be trusted
-    const bool fine = s.y <= 3.0e38f && (fabsf(s.x) <= 3.0e38f || s.y == 0.f);
-    worst = fmaxf(worst, fine ? s.y : INFINITY);
-    if (shared) s_keys[i] = key_of(s.x);
+  for (int i = tid; i < p.error_slots; i += kSelectThreads) {
+    const float e = p.errors[row * p.error_slots + i];
+    fine = fine && e <= 3.0e38f;
+    worst = fmaxf(worst, e);
   }
-  worst = reduce_cta(worst, s_worst, [](float x, float y) { return fmaxf(x, y); });  // s_keys are written, too
-  auto key32 = [&](int64_t i) { return shared ? s_keys[i] : key_of(scores[i].x); };
-  auto inner = [&](int64_t i) { return i > 0 && i < n - 1; };
+  uint32_t least = ~0u, largest = 0u;
+  for (int i = tid; i < n; i += kSelectThreads) {
+    const float s = scores[i];
+    const uint32_t k = key_of(s);
+    fine = fine && s <= 3.0e38f;  // -inf next to finite bounds: a chunk without a block
+    if (shared) s_keys[i] = k;
+    if (inner(i)) {
+      least = min(least, k);
+      largest = max(largest, k);
+    }
+  }
+  if (tid == 0) s_band = 0;
+  const uint32_t off_by = __reduce_max_sync(0xffffffffu, __float_as_uint(fine ? worst : INFINITY));
+  least = __reduce_min_sync(0xffffffffu, least);
+  largest = __reduce_max_sync(0xffffffffu, largest);
+  if (lane == 0) s_range[w] = make_uint4(off_by, least, largest, 0u);
+  __syncthreads();
+  worst = 0.f;
+#pragma unroll
+  for (int j = 0; j < kSelectWarps; ++j) {
+    worst = fmaxf(worst, __uint_as_float(s_range[j].x));
+    least = min(least, s_range[j].y);
+    largest = max(largest, s_range[j].z);
+  }
+  auto key32 = [&](int i) { return shared ? s_keys[i] : key_of(scores[i]); };
   int rest = top - 2;
   float high = INFINITY, low = INFINITY;  // rest = 0: none of the inner chunks
   if (rest > 0) {
     if (worst < INFINITY) {
       int need = rest;
-      const float t = score_of(nth_largest<uint32_t>(n, need, hist, &s_prefix32, &s_need, [&](int64_t i, uint32_t& k) {
+      const int top_bit = 31 - __clz(least ^ largest);  // -1: all alike
+      const uint32_t common = top_bit < 31 ? largest >> (top_bit + 1) : 0u;
+      const float t = score_of(nth_largest<uint32_t>(n, need, top_bit, common, hist, &s_prefix32, &s_need, [&](int i, uint32_t& k) {
         k = key32(i);
         return inner(i);
       }));
@@ -413,49 +438,73 @@ chunk_select_kernel(const SelectParams p) {
       low = -INFINITY;
     }
   }
-  // those certainly in, and those that compete
-  unsigned long long counts = 0;
-  if (rest > 0)
-    for (int64_t i = tid; i < n; i += kSelectThreads)
-      if (inner(i)) {
-        const float s = score_of(key32(i));
-        counts += s > high ? 1ull << 32 : !(s < low) ? 1ull : 0ull;
-      }
-  counts = reduce_cta(counts, s_counts, [](unsigned long long x, unsigned long long y) { return x + y; });
-  const int sure = static_cast<int>(counts >> 32), band = static_cast<int>(counts & 0xffffffffu);
-  const int places = rest - sure;
-  uint64_t bar = 0;     // 64-bit key that a competing chunk has to exceed
-  int equal = band;     // how many of those that reach it are in
-  const bool ranked = band > places;
-  auto competes = [&](int64_t i) {
+  auto competes = [&](int i) {
     const float s = score_of(key32(i));
     return rest > 0 && inner(i) && !(s > high) && !(s < low);
   };
+  // those certainly in, and those that compete
+  unsigned long long counts = 0;
+  if (rest > 0)
+    for (int i = tid; i < n; i += kSelectThreads)
+      if (inner(i)) {
+        const float s = score_of(key32(i));
+        if (s > high) {
+          counts += 1ull << 32;
+        } else if (!(s < low)) {
+          counts += 1ull;
+          const int at = atomicAdd(&s_band, 1);
+          if (at < kSelectBand) band_at[at] = i;
+        }
+      }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) counts += __shfl_xor_sync(0xffffffffu, counts, off);
+  if (lane == 0) s_counts[w] = counts;
+  __syncthreads();
+  counts = 0;
+#pragma unroll
+  for (int j = 0; j < kSelectWarps; ++j) counts += s_counts[j];
+  const int sure = static_cast<int>(counts >> 32), band = static_cast<int>(counts & 0xffffffffu);
+  const int places = rest - sure;
+  const bool ranked = band > places;
+  const bool few = band <= kSelectBand;
+  uint64_t* keys = p.keys + row * p.max_chunks;
+  uint64_t bar = 0;  // many: the 64-bit key that a competing chunk has to exceed,
+  int equal = 0;     // and how many of those that reach it are in
   if (ranked) {
     constexpr int LPC = ScoreLanes<D>::kLanes, CPS = ScoreLanes<D>::kChunks;
     const int kvh = static_cast<int>(row % p.d.num_kv_heads);
     const int32_t* table = p.d.tables + b * p.d.table_stride;
     double wt[8];
     score_weights<T, D>(p, b, kvh, lane, wt);
-    for (int64_t i0 = w * CPS; i0 < n; i0 += kSelectWarps * CPS) {
-      const int64_t i = i0 + lane / LPC;
-      const bool mine = i < n && competes(i);
-      if (!__any_sync(0xffffffffu, mine)) continue;
+    const int candidates = few ? band : n;
+    for (int j0 = w * CPS; j0 < candidates; j0 += kSelectWarps * CPS) {
+      const int j = j0 + lane / LPC;
+      const int i = j >= candidates ? -1 : few ? band_at[j] : competes(j) ? j : -1;
+      if (!__any_sync(0xffffffffu, i >= 0)) continue;
       bool ok = false;
-      const uint4 v = mine ? load_bounds<T, D>(p, table, kvh, i, lane, ok) : zero_vec();
+      const uint4 v = i >= 0 ? load_bounds<T, D>(p, table, kvh, i, lane, ok) : zero_vec();
       float f[8];
       unpack<T>(v, f);
       double s = 0.0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s = fma(wt[j], static_cast<double>(f[j]), s);
+      for (int e = 0; e < 8; ++e) s = fma(wt[e], static_cast<double>(f[e]), s);
 #pragma unroll
       for (int off = LPC / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      if (mine && lane % LPC == 0) keys[i] = ok ? key_of(s) : 0ull;
+      if (i >= 0 && lane % LPC == 0) (few ? band_key[j] : keys[i]) = ok ? key_of(s) : 0ull;
     }
     __syncthreads();
-    int need = places;
-    if (need > 0) {
-      bar = nth_largest<uint64_t>(n, need, hist, &s_prefix64, &s_need, [&](int64_t i, uint64_t& k) {
+    if (few) {
+      if (tid < band) {
+        const uint64_t k = band_key[tid];
+        const int i = band_at[tid];
+        int better = 0;
+        for (int j = 0; j < band; ++j) better += band_key[j] > k || (band_key[j] == k && band_at[j] < i) ? 1 : 0;
+        band_in[tid] = better < places;
+      }
+      __syncthreads();
+    } else if (places > 0) {
+      int need = places;
+      bar = nth_largest<uint64_t>(n, need, 63, 0ull, hist, &s_prefix64, &s_need, [&](int i, uint64_t& k) {
         if (!competes(i)) return false;
         k = keys[i];
         return true;
@@ -463,41 +512,45 @@ chunk_select_kernel(const SelectParams p) {
       equal = need;
     } else {
       bar = ~0ull;
-      equal = 0;
     }
   }
   int done = 0, done_eq = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += kSelectThreads) {
-    const int64_t i = i0 + tid;
+  for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
+    const int i = i0 + tid;
     bool sel = i < n && (!inner(i) || (rest > 0 && score_of(key32(i)) > high));
     bool eq = false;
     if (i < n && competes(i)) {
-      if (ranked) {
-        const uint64_t k = keys[i];
-        sel = k > bar;
-        eq = k == bar;
-      } else {
+      if (!ranked) {
         sel = true;
+      } else if (few) {
+        for (int j = 0; j < band; ++j) sel |= band_at[j] == i && band_in[j];
+      } else {
+        sel = keys[i] > bar;
+        eq = keys[i] == bar;
       }
     }
-    const unsigned eqs = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) warp_eq[w] = __popc(eqs);
-    __syncthreads();
-    int before_eq = done_eq + __popc(eqs & ((1u << lane) - 1));
-    for (int j = 0; j < kSelectWarps; ++j) {
-      if (j < w) before_eq += warp_eq[j];
-      done_eq += warp_eq[j];
+    if (ranked && !few) {  // the lower indices among equals
+      const unsigned eqs = __ballot_sync(0xffffffffu, eq);
+      if (lane == 0) warp_eq[w] = __popc(eqs);
+      __syncthreads();
+      int before = done_eq + __popc(eqs & ((1u << lane) - 1));
+      for (int j = 0; j < kSelectWarps; ++j) {
+        if (j < w) before += warp_eq[j];
+        done_eq += warp_eq[j];
+      }
+      sel = sel || (eq && before < equal);
     }
-    sel = sel || (eq && before_eq < equal);
     const unsigned sels = __ballot_sync(0xffffffffu, sel);
     if (lane == 0) warp_in[w] = __popc(sels);
     __syncthreads();
     int before = done + __popc(sels & ((1u << lane) - 1));
+#pragma unroll
     for (int j = 0; j < kSelectWarps; ++j) {
       if (j < w) before += warp_in[j];
       done += warp_in[j];
     }
-    if (sel) out[before] = static_cast<int32_t>(i);
+    if (sel) out[before] = i;
+    __syncthreads();
   }
 }
 
@@ -506,7 +559,8 @@ chunk_select_kernel(const SelectParams p) {
 struct SparsePlan {
   int splits;
   int64_t max_len, max_chunks;
-  int64_t keys_bytes, partial_bytes;
+  int64_t score_ctas;  // per row
+  int64_t score_bytes, partial_bytes;  // 64-bit keys, scores and errors; partials
 };
 
 static SparsePlan sparse_plan(const nib_sparse_decode_args& s) {
@@ -523,7 +577,12 @@ static SparsePlan sparse_plan(const nib_sparse_decode_args& s) {
   if (n > by_len) n = by_len;
   if (n > 256) n = 256;
   pl.splits = static_cast<int>(n < 1 ? 1 : n);
-  pl.keys_bytes = pl.max_chunks > s.top_chunks ? rows * pl.max_chunks * 16 : 0;
+  // two score CTAs run on an SM: enough of them for two waves, or for all of a row's chunks at once
+  const int64_t per_cta = kScoreWarps * kScoreUnroll * (a.head_dim == 64 ? 2 : 1);
+  const int64_t most = (pl.max_chunks + per_cta - 1) / per_cta;
+  pl.score_ctas = rows < 1 ? 1 : (4LL * sm_count() + rows - 1) / rows;
+  if (pl.score_ctas > most) pl.score_ctas = most;
+  pl.score_bytes = pl.max_chunks > s.top_chunks ? (rows * (pl.max_chunks * 12 + pl.score_ctas * kScoreWarps * 4) + 15) / 16 * 16 : 0;
   pl.partial_bytes = pl.splits > 1 ? nib::partial_bytes(a, pl.splits) : 0;
   return pl;
 }
@@ -537,23 +596,22 @@ static int launch_sparse(const nib_sparse_decode_args& s, const SparsePlan& pl, 
   sp.d.chunk = s.chunk;
   sp.d.top = s.top_chunks;
   sp.d.selected = s.selected;
-  if (pl.splits > 1) place_partials(sp.d, a, static_cast<char*>(a.workspace) + pl.keys_bytes);
+  if (pl.splits > 1) place_partials(sp.d, a, static_cast<char*>(a.workspace) + pl.score_bytes);
   sp.bounds = s.bounds;
   sp.b_bs = s.bounds_block_stride;
   sp.b_hs = s.bounds_head_stride;
   const int64_t rows = a.batch * a.num_kv_heads;
-  sp.scores = static_cast<float2*>(a.workspace);
-  sp.keys = reinterpret_cast<uint64_t*>(sp.scores + rows * pl.max_chunks);
+  sp.keys = static_cast<uint64_t*>(a.workspace);
+  sp.scores = reinterpret_cast<float*>(sp.keys + rows * pl.max_chunks);
+  sp.errors = sp.scores + rows * pl.max_chunks;
+  sp.error_slots = static_cast<int>(pl.score_ctas) * kScoreWarps;
   sp.max_chunks = pl.max_chunks;
   sp.selected = s.selected;
-  if (pl.keys_bytes > 0) {
-    // two CTAs run on an SM: enough of them for two waves, or for all of a row's chunks at once
-    constexpr int kChunks = kScoreWarps * kScoreUnroll * ScoreLanes<D>::kChunks;
-    const int64_t most = (pl.max_chunks + kChunks - 1) / kChunks, want = (4LL * sm_count() + rows - 1) / rows;
-    const dim3 grid(static_cast<unsigned>(most < want ? most : want), static_cast<unsigned>(rows));
+  if (pl.score_bytes > 0) {
+    const dim3 grid(static_cast<unsigned>(pl.score_ctas), static_cast<unsigned>(rows));
     launch_k(chunk_score_kernel<T, D>, grid, kScoreWarps * 32, 0, st, sp);
   }
-  launch_k_pdl(pl.keys_bytes > 0 || pdl_enabled(), chunk_select_kernel<T, D>, static_cast<unsigned>(rows), kSelectThreads, 0, st, sp);
+  launch_k_pdl(pl.score_bytes > 0 || pdl_enabled(), chunk_select_kernel<T, D>, static_cast<unsigned>(rows), kSelectThreads, 0, st, sp);
   const int rc = launch_mma_mode<T, D, kDecodeSparse>(a, sp.d, rows, st, true);
   if (rc != NIB_OK || pl.splits == 1) return rc;
   return launch_combine_partials<T, D, kDecodeSparse>(a, sp.d, st);
@@ -629,7 +687,7 @@ extern "C" int nib_paged_key_bounds(int dtype, const void* key_cache, int64_t ca
 extern "C" int64_t nib_sparse_decode_workspace_bytes(const nib_sparse_decode_args* s) {
   if (sparse_check(s) != nullptr) return -1;
   const SparsePlan pl = sparse_plan(*s);
-  return pl.keys_bytes + pl.partial_bytes;
+  return pl.score_bytes + pl.partial_bytes;
 }
 
 extern "C" int nib_sparse_decode_attention(const nib_sparse_decode_args* s, void* stream) {
@@ -651,7 +709,7 @@ extern "C" int nib_sparse_decode_attention(const nib_sparse_decode_args* s, void
   NIB_SUPPORT(decode_mma_eligible(a), "sparse_decode_attention: needs bf16/f16, head_dim 64 or 128, at most 16 q "
               "heads per kv head, a block size that is a multiple of 16 and 16-byte aligned strides");
   const SparsePlan pl = sparse_plan(*s);
-  const int64_t need = pl.keys_bytes + pl.partial_bytes;
+  const int64_t need = pl.score_bytes + pl.partial_bytes;
   NIB_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= need && aligned16(a.workspace)),
               "sparse_decode_attention: workspace of %lld bytes needed", static_cast<long long>(need));
   const cudaStream_t st = as_stream(stream);
