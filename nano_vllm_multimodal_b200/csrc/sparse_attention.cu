@@ -137,6 +137,7 @@ struct SelectParams {
   uint64_t* keys;      // as many as scores: the chunks that are scored in 64 bits
   int64_t max_chunks;
   int error_slots;
+  int per, per_shift;  // chunks per block; its log2 where it is a power of two, else -1
   int32_t* selected;   // [batch * kv heads, top]
 };
 
@@ -166,27 +167,33 @@ __device__ __forceinline__ void score_weights(const SelectParams& p, int64_t b, 
   }
 }
 
+// chunk c's block in its table and its place there
+__device__ __forceinline__ int2 chunk_place(const SelectParams& p, int c) {
+  if (p.per_shift >= 0) return make_int2(c >> p.per_shift, c & (p.per - 1));
+  return make_int2(c / p.per, c % p.per);
+}
+
 // the lane's 16 bytes of chunk c, zeros where its block does not exist
 template <typename T, int D>
-__device__ __forceinline__ uint4 load_bounds(const SelectParams& p, const int32_t* table, int kvh, int64_t c, int lane, bool& ok) {
+__device__ __forceinline__ uint4 load_bounds(const SelectParams& p, const int32_t* table, int kvh, int c, int lane, bool& ok) {
   constexpr int half = ScoreLanes<D>::kLanes / 2;
   const int part = lane % ScoreLanes<D>::kLanes;
-  const int per = p.d.block_size / p.d.chunk;
-  const int blk = __ldg(table + c / per);
+  const int2 at = chunk_place(p, c);
+  const int blk = __ldg(table + at.x);
   ok = blk >= 0 && blk < p.d.num_blocks;
   if (!ok) return zero_vec();
-  return ld_stream(static_cast<const T*>(p.bounds) + blk * p.b_bs + kvh * p.b_hs + ((c % per) * 2 + (part >= half ? 1 : 0)) * D +
+  return ld_stream(static_cast<const T*>(p.bounds) + blk * p.b_bs + kvh * p.b_hs + (at.y * 2 + (part >= half ? 1 : 0)) * D +
                    (part % half) * 8);
 }
 
 constexpr int kScoreWarps = 8;
 constexpr int kScoreUnroll = 8;
 
-// Scores in 32 bits. Error: a weight is rounded once, a lane adds 8 products with fused
-// operations, five shuffles add the lanes: at most 14 roundings of 2^-24 relative to the sum of
-// the terms' absolute values. A warp bounds that sum for all of its chunks at once, by the largest
-// |value| of each channel; the bound's own sum is 2^-20 off at most, so 1.25 * 2^-20 of it covers
-// the error, and 2^-126 terms too small for relative errors.
+// Scores in 32 bits. Error: a weight is a sum of at most 16 terms of one sign, a lane adds 8
+// products with fused operations, five shuffles add the lanes: at most 15 + 8 + 5 roundings of
+// 2^-24 relative to the sum of the terms' absolute values. A warp bounds that sum for all of its
+// chunks at once, by the largest |value| of each channel; the bound's own sum is 2^-19 off at
+// most, so 1.25 * 2^-19 of it covers the error, and 2^-126 terms too small for relative errors.
 //
 // A warp takes every gridDim.x * kScoreWarps-th group of kScoreUnroll steps of a row (4 KB of
 // bounds) and loads the next group before it works on this one.
@@ -211,14 +218,14 @@ chunk_score_kernel(const SelectParams p) {
     return;
   }
   const int32_t* table = p.d.tables + b * p.d.table_stride;
-  const int per = p.d.block_size / p.d.chunk;
   const int part = lane % LPC;
   const T* base = static_cast<const T*>(p.bounds) + kvh * p.b_hs + (part >= half ? D : 0) + (part % half) * 8;
   // lane j looks chunk c0 + j of a group up: its block and its place there, -1 for none
   auto look_up = [&](int c) -> int2 {
     if (lane >= G || c + lane >= chunks) return make_int2(-1, 0);
-    const int blk = __ldg(table + (c + lane) / per);
-    if (blk >= 0 && blk < p.d.num_blocks) return make_int2(blk, (c + lane) % per);
+    const int2 at = chunk_place(p, c + lane);
+    const int blk = __ldg(table + at.x);
+    if (blk >= 0 && blk < p.d.num_blocks) return make_int2(blk, at.y);
     flag(p.d.status, NIB_DEV_BAD_BLOCK);
     return make_int2(-1, 0);
   };
@@ -236,12 +243,24 @@ chunk_score_kernel(const SelectParams p) {
   unsigned have;
   load(look_up(c0), v, have);
   int2 next_place = look_up(c0 + step);
-  float wt[8];
-  {
-    double exact[8];
-    score_weights<T, D>(p, b, kvh, lane, exact);
+  // the weights, with both signs as positive parts; a query that is not finite makes them NaN
+  float wt[8], odd = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) wt[i] = static_cast<float>(exact[i]);
+  for (int i = 0; i < 8; ++i) wt[i] = 0.f;
+  {
+    const float sign = part >= half ? 1.f : -1.f;
+    const T* q = static_cast<const T*>(p.d.q) + b * p.d.q_bs + kvh * p.d.group * p.d.q_hs + (part % half) * 8;
+    for (int h = 0; h < p.d.group; ++h) {
+      float f[8];
+      unpack<T>(ld_vec(q + h * p.d.q_hs), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        wt[i] += fmaxf(f[i] * sign, 0.f);
+        odd = fmaf(f[i], 0.f, odd);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wt[i] = fmaf(wt[i], sign, odd);
   }
   float* out = p.scores + row * p.max_chunks;
   float most[8];
@@ -277,7 +296,7 @@ chunk_score_kernel(const SelectParams p) {
 #pragma unroll
   for (int off = LPC / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if (CPS == 2) sum = fmaxf(sum, __shfl_xor_sync(0xffffffffu, sum, 16)) + (sum - sum);  // a NaN stays one
-  if (lane == 0) *error = fmaf(sum, 1.25f * 9.5367431640625e-7f, 1.1754943508222875e-38f);
+  if (lane == 0) *error = fmaf(sum, 1.25f * 1.9073486328125e-6f, 1.1754943508222875e-38f);
 }
 
 // A 32-bit score as a whole number of the same order (-0 as 0).
@@ -301,55 +320,112 @@ constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectShared = 8192;  // chunks whose 32-bit keys are kept in shared memory
 constexpr int kSelectBand = 256;     // competing chunks that are ranked by comparing each with each
 
-// The need-th largest of the keys that key(i, k) yields for i < n (false: i takes no part), eight
-// bits at a time from bit `top_bit` down (above it all keys are those of `prefix`); need becomes
-// how many of those equal to it are among the first need. By the whole CTA.
-template <typename K, typename F>
-__device__ __forceinline__ K nth_largest(int n, int& need, int top_bit, K prefix, unsigned int* hist, K* s_prefix,
-                                         int* s_need, F key) {
-  static_assert(kSelectThreads == 256, "a thread per bin");
+struct SelectShared {
+  uint32_t keys[kSelectShared];
+  unsigned int hist[256];
+  uint64_t member[kSelectBand], found;
+  int digit, need, members;
+  int at[kSelectBand];
+  uint64_t key[kSelectBand];
+  bool in[kSelectBand];
+  uint4 range[kSelectWarps];
+  unsigned long long counts[kSelectWarps];
+  int sums[kSelectWarps];
+  int band;
+};
+
+// The need-th largest of the keys that key(i, k) yields for i < n (false: i takes no part), from
+// bit `top_bit` down (above it all keys are those of `prefix`); need becomes how many of those
+// equal to it are among the first need. By the whole CTA: eight bits at a time by counting, until
+// the keys that share the bits so far are few enough to compare each with each.
+template <typename F>
+__device__ __forceinline__ uint64_t nth_largest(SelectShared& s, int n, int& need, int top_bit, uint64_t prefix, F key) {
+  static_assert(kSelectThreads == 256 && kSelectBand == 256, "a thread per bin and per member");
   const int tid = threadIdx.x, lane = tid & 31;
   int done = top_bit + 1;  // bits still open
   while (done > 0) {
     const int bits = done < 8 ? done : 8, shift = done - bits;
-    hist[tid] = 0;
+    s.hist[tid] = 0;
+    if (tid == 0) s.members = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-      K k = 0;
-      if (i0 + tid < n && key(i0 + tid, k) && (k >> (shift + bits - 1)) >> 1 == prefix)
-        atomicAdd(&hist[static_cast<int>(k >> shift) & ((1 << bits) - 1)], 1u);
+    for (int i = tid; i < n; i += kSelectThreads) {
+      uint64_t k;
+      if (key(i, k) && (k >> (shift + bits - 1)) >> 1 == prefix)
+        atomicAdd(&s.hist[static_cast<int>(k >> shift) & ((1 << bits) - 1)], 1u);
     }
     __syncthreads();
     if (tid < 32) {  // lane l: bins 255 - 8 l down to 248 - 8 l
-      int mine = 0;
+      int count[8], mine = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mine += static_cast<int>(hist[255 - 8 * lane - j]);
+      for (int j = 0; j < 8; ++j) {
+        count[j] = static_cast<int>(s.hist[255 - 8 * lane - j]);
+        mine += count[j];
+      }
       int upto = mine;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, off);
         if (lane >= off) upto += v;
       }
-      const unsigned reach = __ballot_sync(0xffffffffu, upto >= need);
-      if (lane == __ffs(reach) - 1) {
-        int above = upto - mine;
-        for (int j = 0; j < 8; ++j) {
-          const int bin = 255 - 8 * lane - j;
-          if (above + static_cast<int>(hist[bin]) >= need) {
-            *s_prefix = (prefix << bits) | static_cast<K>(bin);
-            *s_need = need - above;
-            break;
-          }
-          above += static_cast<int>(hist[bin]);
+      int above = upto - mine;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (above < need && above + count[j] >= need) {  // true for one bin of all
+          s.digit = 255 - 8 * lane - j;
+          s.need = need - above;
+          s.band = count[j];
         }
+        above += count[j];
       }
     }
     __syncthreads();
-    prefix = *s_prefix;
-    need = *s_need;
+    prefix = (prefix << bits) | static_cast<uint64_t>(s.digit);
+    need = s.need;
     done = shift;
+    if (s.band <= kSelectBand) {
+      for (int i = tid; i < n; i += kSelectThreads) {
+        uint64_t k;
+        if (key(i, k) && k >> shift == prefix) s.member[atomicAdd(&s.members, 1)] = k;
+      }
+      __syncthreads();
+      const int m = s.members;
+      if (tid < m) {
+        const uint64_t k = s.member[tid];
+        int greater = 0, same = 0;
+        for (int j = 0; j < m; ++j) {
+          greater += s.member[j] > k ? 1 : 0;
+          same += s.member[j] == k ? 1 : 0;
+        }
+        if (greater < need && need <= greater + same) {  // the same for all that hold this key
+          s.found = k;
+          s.need = need - greater;
+        }
+      }
+      __syncthreads();
+      prefix = s.found;
+      need = s.need;
+      break;
+    }
   }
   return prefix;
+}
+
+// exclusive prefix sum over the CTA's threads
+__device__ __forceinline__ int scan_threads(SelectShared& s, int v) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int upto = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += x;
+  }
+  __syncthreads();
+  if (lane == 31) s.sums[w] = upto;
+  __syncthreads();
+  int before = upto - v;
+#pragma unroll
+  for (int j = 0; j < kSelectWarps; ++j) before += j < w ? s.sums[j] : 0;
+  return before;
 }
 
 // The `top` best chunks of a row, in ascending order of index. The first and the last chunk are
@@ -361,15 +437,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kSelectThreads)
 chunk_select_kernel(const SelectParams p) {
   pdl_enter();
-  __shared__ uint32_t s_keys[kSelectShared];
-  __shared__ unsigned int hist[256];
-  __shared__ uint64_t s_prefix64, band_key[kSelectBand];
-  __shared__ uint32_t s_prefix32;
-  __shared__ int s_need, s_band, band_at[kSelectBand];
-  __shared__ bool band_in[kSelectBand];
-  __shared__ uint4 s_range[kSelectWarps];
-  __shared__ unsigned long long s_counts[kSelectWarps];
-  __shared__ int warp_in[kSelectWarps], warp_eq[kSelectWarps];
+  __shared__ SelectShared s;
   const int64_t row = blockIdx.x;
   const int64_t b = row / p.d.num_kv_heads;
   const int64_t len = clamped_len(p.d, b, false);
@@ -395,29 +463,28 @@ chunk_select_kernel(const SelectParams p) {
   }
   uint32_t least = ~0u, largest = 0u;
   for (int i = tid; i < n; i += kSelectThreads) {
-    const float s = scores[i];
-    const uint32_t k = key_of(s);
-    fine = fine && s <= 3.0e38f;  // -inf next to finite bounds: a chunk without a block
-    if (shared) s_keys[i] = k;
+    const float x = scores[i];
+    const uint32_t k = key_of(x);
+    fine = fine && x <= 3.0e38f;  // -inf next to finite bounds: a chunk without a block
+    if (shared) s.keys[i] = k;
     if (inner(i)) {
       least = min(least, k);
       largest = max(largest, k);
     }
   }
-  if (tid == 0) s_band = 0;
   const uint32_t off_by = __reduce_max_sync(0xffffffffu, __float_as_uint(fine ? worst : INFINITY));
   least = __reduce_min_sync(0xffffffffu, least);
   largest = __reduce_max_sync(0xffffffffu, largest);
-  if (lane == 0) s_range[w] = make_uint4(off_by, least, largest, 0u);
+  if (lane == 0) s.range[w] = make_uint4(off_by, least, largest, 0u);
   __syncthreads();
   worst = 0.f;
 #pragma unroll
   for (int j = 0; j < kSelectWarps; ++j) {
-    worst = fmaxf(worst, __uint_as_float(s_range[j].x));
-    least = min(least, s_range[j].y);
-    largest = max(largest, s_range[j].z);
+    worst = fmaxf(worst, __uint_as_float(s.range[j].x));
+    least = min(least, s.range[j].y);
+    largest = max(largest, s.range[j].z);
   }
-  auto key32 = [&](int i) { return shared ? s_keys[i] : key_of(scores[i]); };
+  auto key32 = [&](int i) { return shared ? s.keys[i] : key_of(scores[i]); };
   int rest = top - 2;
   float high = INFINITY, low = INFINITY;  // rest = 0: none of the inner chunks
   if (rest > 0) {
@@ -425,10 +492,10 @@ chunk_select_kernel(const SelectParams p) {
       int need = rest;
       const int top_bit = 31 - __clz(least ^ largest);  // -1: all alike
       const uint32_t common = top_bit < 31 ? largest >> (top_bit + 1) : 0u;
-      const float t = score_of(nth_largest<uint32_t>(n, need, top_bit, common, hist, &s_prefix32, &s_need, [&](int i, uint32_t& k) {
+      const float t = score_of(static_cast<uint32_t>(nth_largest(s, n, need, top_bit, common, [&](int i, uint64_t& k) {
         k = key32(i);
         return inner(i);
-      }));
+      })));
       // rounded outwards
       high = t + 2.f * worst;
       low = t - 2.f * worst;
@@ -439,30 +506,33 @@ chunk_select_kernel(const SelectParams p) {
     }
   }
   auto competes = [&](int i) {
-    const float s = score_of(key32(i));
-    return rest > 0 && inner(i) && !(s > high) && !(s < low);
+    const float x = score_of(key32(i));
+    return rest > 0 && inner(i) && !(x > high) && !(x < low);
   };
   // those certainly in, and those that compete
+  __syncthreads();
+  if (tid == 0) s.band = 0;
+  __syncthreads();
   unsigned long long counts = 0;
   if (rest > 0)
     for (int i = tid; i < n; i += kSelectThreads)
       if (inner(i)) {
-        const float s = score_of(key32(i));
-        if (s > high) {
+        const float x = score_of(key32(i));
+        if (x > high) {
           counts += 1ull << 32;
-        } else if (!(s < low)) {
+        } else if (!(x < low)) {
           counts += 1ull;
-          const int at = atomicAdd(&s_band, 1);
-          if (at < kSelectBand) band_at[at] = i;
+          const int at = atomicAdd(&s.band, 1);
+          if (at < kSelectBand) s.at[at] = i;
         }
       }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) counts += __shfl_xor_sync(0xffffffffu, counts, off);
-  if (lane == 0) s_counts[w] = counts;
+  if (lane == 0) s.counts[w] = counts;
   __syncthreads();
   counts = 0;
 #pragma unroll
-  for (int j = 0; j < kSelectWarps; ++j) counts += s_counts[j];
+  for (int j = 0; j < kSelectWarps; ++j) counts += s.counts[j];
   const int sure = static_cast<int>(counts >> 32), band = static_cast<int>(counts & 0xffffffffu);
   const int places = rest - sure;
   const bool ranked = band > places;
@@ -479,32 +549,32 @@ chunk_select_kernel(const SelectParams p) {
     const int candidates = few ? band : n;
     for (int j0 = w * CPS; j0 < candidates; j0 += kSelectWarps * CPS) {
       const int j = j0 + lane / LPC;
-      const int i = j >= candidates ? -1 : few ? band_at[j] : competes(j) ? j : -1;
+      const int i = j >= candidates ? -1 : few ? s.at[j] : competes(j) ? j : -1;
       if (!__any_sync(0xffffffffu, i >= 0)) continue;
       bool ok = false;
       const uint4 v = i >= 0 ? load_bounds<T, D>(p, table, kvh, i, lane, ok) : zero_vec();
       float f[8];
       unpack<T>(v, f);
-      double s = 0.0;
+      double x = 0.0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fma(wt[e], static_cast<double>(f[e]), s);
+      for (int e = 0; e < 8; ++e) x = fma(wt[e], static_cast<double>(f[e]), x);
 #pragma unroll
-      for (int off = LPC / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      if (i >= 0 && lane % LPC == 0) (few ? band_key[j] : keys[i]) = ok ? key_of(s) : 0ull;
+      for (int off = LPC / 2; off >= 1; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+      if (i >= 0 && lane % LPC == 0) (few ? s.key[j] : keys[i]) = ok ? key_of(x) : 0ull;
     }
     __syncthreads();
     if (few) {
       if (tid < band) {
-        const uint64_t k = band_key[tid];
-        const int i = band_at[tid];
+        const uint64_t k = s.key[tid];
+        const int i = s.at[tid];
         int better = 0;
-        for (int j = 0; j < band; ++j) better += band_key[j] > k || (band_key[j] == k && band_at[j] < i) ? 1 : 0;
-        band_in[tid] = better < places;
+        for (int j = 0; j < band; ++j) better += s.key[j] > k || (s.key[j] == k && s.at[j] < i) ? 1 : 0;
+        s.in[tid] = better < places;
       }
       __syncthreads();
     } else if (places > 0) {
       int need = places;
-      bar = nth_largest<uint64_t>(n, need, 63, 0ull, hist, &s_prefix64, &s_need, [&](int i, uint64_t& k) {
+      bar = nth_largest(s, n, need, 63, 0ull, [&](int i, uint64_t& k) {
         if (!competes(i)) return false;
         k = keys[i];
         return true;
@@ -514,44 +584,32 @@ chunk_select_kernel(const SelectParams p) {
       bar = ~0ull;
     }
   }
-  int done = 0, done_eq = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    bool sel = i < n && (!inner(i) || (rest > 0 && score_of(key32(i)) > high));
-    bool eq = false;
-    if (i < n && competes(i)) {
-      if (!ranked) {
-        sel = true;
-      } else if (few) {
-        for (int j = 0; j < band; ++j) sel |= band_at[j] == i && band_in[j];
-      } else {
-        sel = keys[i] > bar;
-        eq = keys[i] == bar;
-      }
-    }
-    if (ranked && !few) {  // the lower indices among equals
-      const unsigned eqs = __ballot_sync(0xffffffffu, eq);
-      if (lane == 0) warp_eq[w] = __popc(eqs);
-      __syncthreads();
-      int before = done_eq + __popc(eqs & ((1u << lane) - 1));
-      for (int j = 0; j < kSelectWarps; ++j) {
-        if (j < w) before += warp_eq[j];
-        done_eq += warp_eq[j];
-      }
-      sel = sel || (eq && before < equal);
-    }
-    const unsigned sels = __ballot_sync(0xffffffffu, sel);
-    if (lane == 0) warp_in[w] = __popc(sels);
-    __syncthreads();
-    int before = done + __popc(sels & ((1u << lane) - 1));
-#pragma unroll
-    for (int j = 0; j < kSelectWarps; ++j) {
-      if (j < w) before += warp_in[j];
-      done += warp_in[j];
-    }
-    if (sel) out[before] = i;
-    __syncthreads();
+  // each thread's share of consecutive chunks, in order: `left` of the equal ones are still to take
+  const int share = (n + kSelectThreads - 1) / kSelectThreads;
+  const int from = tid * share, to = from + share < n ? from + share : n;
+  int left = 0;
+  if (ranked && !few) {
+    int same = 0;
+    for (int i = from; i < to; ++i) same += competes(i) && keys[i] == bar ? 1 : 0;
+    left = equal - scan_threads(s, same);
   }
+  auto selected = [&](int i, int& left) {
+    if (!inner(i)) return true;
+    const float x = score_of(key32(i));
+    if (rest <= 0 || x < low) return false;
+    if (x > high || !ranked) return true;
+    if (few) {
+      bool in = false;
+      for (int j = 0; j < band; ++j) in |= s.at[j] == i && s.in[j];
+      return in;
+    }
+    return keys[i] > bar || (keys[i] == bar && left-- > 0);
+  };
+  int mine = 0, still = left;
+  for (int i = from; i < to; ++i) mine += selected(i, still) ? 1 : 0;
+  int at = scan_threads(s, mine);
+  for (int i = from; i < to; ++i)
+    if (selected(i, left)) out[at++] = i;
 }
 
 // ------------------------------------------------------------------ host side
@@ -605,6 +663,10 @@ static int launch_sparse(const nib_sparse_decode_args& s, const SparsePlan& pl, 
   sp.scores = reinterpret_cast<float*>(sp.keys + rows * pl.max_chunks);
   sp.errors = sp.scores + rows * pl.max_chunks;
   sp.error_slots = static_cast<int>(pl.score_ctas) * kScoreWarps;
+  sp.per = static_cast<int>(a.block_size / s.chunk);
+  sp.per_shift = -1;
+  for (int k = 0; k < 31; ++k)
+    if ((1 << k) == sp.per) sp.per_shift = k;
   sp.max_chunks = pl.max_chunks;
   sp.selected = s.selected;
   if (pl.score_bytes > 0) {
