@@ -8,9 +8,9 @@
 //   score(chunk) = a . hi + b . lo,   a = sum_h q_h+,   b = sum_h q_h-
 // bounds the sum of the heads' scores from above with one dot product of 2 D terms, whatever
 // the number of heads. Chunks are ranked by their scores in 64 bits (in 32, the order of the
-// summation would decide between near neighbours), yet hardly any is computed so: the score
-// kernel sums in 32 bits and bounds its own error, and the selection repeats in 64 bits only the
-// chunks that the bound leaves within reach of the last place - mostly none.
+// summation would decide between near neighbours), yet hardly any is computed so: scores are
+// summed in 32 bits with a bound of their error, and only the chunks that the bound leaves within
+// reach of the last place - mostly none - are scored again in 64 bits.
 #include "decode_mma.cuh"
 
 namespace nib {
@@ -188,68 +188,47 @@ __device__ __forceinline__ uint4 load_bounds(const SelectParams& p, const int32_
 
 constexpr int kScoreWarps = 8;
 constexpr int kScoreUnroll = 8;
+constexpr int kScoreResident = 4;  // CTAs per SM that the registers are sized for
 
-// Scores in 32 bits. Error: a weight is a sum of at most 16 terms of one sign, a lane adds 8
-// products with fused operations, five shuffles add the lanes: at most 15 + 8 + 5 roundings of
-// 2^-24 relative to the sum of the terms' absolute values. A warp bounds that sum for all of its
-// chunks at once, by the largest |value| of each channel; the bound's own sum is 2^-19 off at
-// most, so 1.25 * 2^-19 of it covers the error, and 2^-126 terms too small for relative errors.
+// Scores of a row's chunks in 32 bits, by one of `parts` CTAs. Error: a weight is a sum of at most
+// 16 terms of one sign, a lane adds 8 products with fused operations, five shuffles add the lanes:
+// at most 15 + 8 + 5 roundings of 2^-24 relative to the sum of the terms' absolute values. A warp
+// bounds that sum for all of its chunks at once, by the largest |value| of each channel; the
+// bound's own sum is 2^-19 off at most, so 1.25 * 2^-19 of it covers the error, and 2^-126 terms
+// too small for relative errors.
 //
-// A warp takes every gridDim.x * kScoreWarps-th group of kScoreUnroll steps of a row (4 KB of
-// bounds) and loads the next group before it works on this one.
+// A warp takes groups of kScoreUnroll steps (4 KB of bounds), all loads of a group in flight. The
+// lanes' sums of eight steps are added by halving: each exchange halves the steps that a lane is
+// left with (9 shuffles for 8 chunks of 32 lanes, not 40).
 template <typename T, int D>
-__global__ void __launch_bounds__(kScoreWarps * 32, 2)
-chunk_score_kernel(const SelectParams p) {
-  pdl_enter();
+__device__ __forceinline__ void score_chunks(const SelectParams& p, int64_t row, int64_t b, int kvh, int chunks, int part_of,
+                                             int parts) {
   constexpr int LPC = ScoreLanes<D>::kLanes, CPS = ScoreLanes<D>::kChunks, G = kScoreUnroll * CPS;
   constexpr int half = LPC / 2;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t row = blockIdx.y;
-  const int64_t b = row / p.d.num_kv_heads;
-  const int kvh = static_cast<int>(row % p.d.num_kv_heads);
-  const int64_t len = clamped_len(p.d, b, threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0);
-  const int chunks = static_cast<int>((len + p.d.chunk - 1) / p.d.chunk);
-  const int step = static_cast<int>(gridDim.x) * kScoreWarps * G;
-  int c0 = (static_cast<int>(blockIdx.x) * kScoreWarps + w) * G;
-  if (chunks <= p.d.top) return;  // all of them are selected
-  float* error = p.errors + row * p.error_slots + blockIdx.x * kScoreWarps + w;
-  if (c0 >= chunks) {
-    if (lane == 0) *error = 0.f;
-    return;
-  }
-  const int32_t* table = p.d.tables + b * p.d.table_stride;
+  const int step = parts * kScoreWarps * G;
+  int c0 = (part_of * kScoreWarps + w) * G;
   const int part = lane % LPC;
+  const int32_t* table = p.d.tables + b * p.d.table_stride;
   const T* base = static_cast<const T*>(p.bounds) + kvh * p.b_hs + (part >= half ? D : 0) + (part % half) * 8;
-  // lane j looks chunk c0 + j of a group up: its block and its place there, -1 for none
-  auto look_up = [&](int c) -> int2 {
-    if (lane >= G || c + lane >= chunks) return make_int2(-1, 0);
+  // lane j looks chunk c + j of a group up: where its bounds begin, -1: it has none
+  auto look_up = [&](int c) -> int64_t {
+    if (lane >= G || c + lane >= chunks) return -1;
     const int2 at = chunk_place(p, c + lane);
     const int blk = __ldg(table + at.x);
-    if (blk >= 0 && blk < p.d.num_blocks) return make_int2(blk, at.y);
+    if (blk >= 0 && blk < p.d.num_blocks) return blk * p.b_bs + at.y * 2 * D;
     flag(p.d.status, NIB_DEV_BAD_BLOCK);
-    return make_int2(-1, 0);
+    return -1;
   };
-  auto load = [&](int2 place, uint4 (&v)[kScoreUnroll], unsigned& have) {
-    have = __ballot_sync(0xffffffffu, place.x >= 0);
-#pragma unroll
-    for (int j = 0; j < kScoreUnroll; ++j) {
-      const int blk = __shfl_sync(0xffffffffu, place.x, j * CPS + lane / LPC);
-      const int at = __shfl_sync(0xffffffffu, place.y, j * CPS + lane / LPC);
-      v[j] = zero_vec();
-      if (blk >= 0) v[j] = ld_stream(base + blk * p.b_bs + at * 2 * D);
-    }
-  };
-  uint4 v[kScoreUnroll];
-  unsigned have;
-  load(look_up(c0), v, have);
-  int2 next_place = look_up(c0 + step);
+  int64_t place = look_up(c0);
   // the weights, with both signs as positive parts; a query that is not finite makes them NaN
-  float wt[8], odd = 0.f;
+  float wt[8], most[8], odd = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) wt[i] = 0.f;
+  for (int i = 0; i < 8; ++i) wt[i] = most[i] = 0.f;
   {
     const float sign = part >= half ? 1.f : -1.f;
     const T* q = static_cast<const T*>(p.d.q) + b * p.d.q_bs + kvh * p.d.group * p.d.q_hs + (part % half) * 8;
+#pragma unroll 4
     for (int h = 0; h < p.d.group; ++h) {
       float f[8];
       unpack<T>(ld_vec(q + h * p.d.q_hs), f);
@@ -263,32 +242,44 @@ chunk_score_kernel(const SelectParams p) {
     for (int i = 0; i < 8; ++i) wt[i] = fmaf(wt[i], sign, odd);
   }
   float* out = p.scores + row * p.max_chunks;
-  float most[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) most[i] = 0.f;
   for (; c0 < chunks; c0 += step) {
-    uint4 next[kScoreUnroll];
-    unsigned next_have;
-    load(next_place, next, next_have);
-    next_place = look_up(c0 + 2 * step);
+    uint4 v[kScoreUnroll];
+    const unsigned have = __ballot_sync(0xffffffffu, place >= 0);
+#pragma unroll
+    for (int j = 0; j < kScoreUnroll; ++j) {
+      const int64_t at = __shfl_sync(0xffffffffu, place, j * CPS + lane / LPC);
+      v[j] = zero_vec();
+      if (at >= 0) v[j] = ld_stream(base + at);
+    }
+    place = look_up(c0 + step);
+    float s[kScoreUnroll];
 #pragma unroll
     for (int j = 0; j < kScoreUnroll; ++j) {
       float f[8];
       unpack<T>(v[j], f);
-      float s = 0.f;
+      s[j] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        s = fmaf(wt[i], f[i], s);
+        s[j] = fmaf(wt[i], f[i], s[j]);
         most[i] = fmaxf(most[i], fabsf(f[i]));
       }
-#pragma unroll
-      for (int off = LPC / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      const int c = c0 + j * CPS + lane / LPC;
-      // a chunk without a block ranks below every other (two of them by their index)
-      if (part == 0 && c < chunks) out[c] = (have >> (j * CPS + lane / LPC)) & 1u ? s : -INFINITY;
-      v[j] = next[j];
     }
-    have = next_have;
+    int mine = 0;  // the step that this lane is left with
+#pragma unroll
+    for (int n = kScoreUnroll / 2, off = LPC / 2; n >= 1; n /= 2, off /= 2) {
+      const bool upper = (lane & off) != 0;
+      mine += upper ? n : 0;
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        const float keep = upper ? s[j + n] : s[j], give = upper ? s[j] : s[j + n];
+        s[j] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+      }
+    }
+#pragma unroll
+    for (int off = LPC / 16; off >= 1; off /= 2) s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
+    const int c = mine * CPS + lane / LPC;
+    // a chunk without a block ranks below every other (two of them by their index)
+    if ((lane & (LPC / 8 - 1)) == 0 && c0 + c < chunks) out[c0 + c] = (have >> c) & 1u ? s[0] : -INFINITY;
   }
   float sum = 0.f;
 #pragma unroll
@@ -296,7 +287,8 @@ chunk_score_kernel(const SelectParams p) {
 #pragma unroll
   for (int off = LPC / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if (CPS == 2) sum = fmaxf(sum, __shfl_xor_sync(0xffffffffu, sum, 16)) + (sum - sum);  // a NaN stays one
-  if (lane == 0) *error = fmaf(sum, 1.25f * 1.9073486328125e-6f, 1.1754943508222875e-38f);
+  if (lane == 0)
+    p.errors[row * p.error_slots + part_of * kScoreWarps + w] = fmaf(sum, 1.25f * 1.9073486328125e-6f, 1.1754943508222875e-38f);
 }
 
 // A 32-bit score as a whole number of the same order (-0 as 0).
@@ -428,27 +420,36 @@ __device__ __forceinline__ int scan_threads(SelectShared& s, int v) {
   return before;
 }
 
-// The `top` best chunks of a row, in ascending order of index. The first and the last chunk are
+// The `top` best chunks of a row, in ascending order of index: the CTAs of a cluster score the
+// row's chunks by turns, then the first of them selects (the others end, and with them their
+// SMs are free for other rows). The first and the last chunk are
 // in; `rest` others are wanted. With T the rest-th largest 32-bit score and E the row's largest
 // error bound, a chunk above T + 2 E is in for certain, one below T - 2 E out, and those between
 // compete in 64 bits for the places that are left (unless the places suffice for all of them).
 // A score or bound that is not finite makes E infinite: then every chunk competes.
 template <typename T, int D>
-__global__ void __launch_bounds__(kSelectThreads)
+__global__ void __launch_bounds__(kSelectThreads, kScoreResident)
 chunk_select_kernel(const SelectParams p) {
+  static_assert(kSelectThreads == kScoreWarps * 32, "the same CTA scores and selects");
   pdl_enter();
   __shared__ SelectShared s;
-  const int64_t row = blockIdx.x;
+  const int64_t row = blockIdx.y;
   const int64_t b = row / p.d.num_kv_heads;
-  const int64_t len = clamped_len(p.d, b, false);
+  const int kvh = static_cast<int>(row % p.d.num_kv_heads);
+  const int64_t len = clamped_len(p.d, b, threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0);
   const int n = static_cast<int>((len + p.d.chunk - 1) / p.d.chunk);
   const int top = p.d.top;
   int32_t* out = p.selected + row * top;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  if (n <= top) {
-    for (int i = tid; i < top; i += kSelectThreads) out[i] = i < n ? i : -1;
+  if (n <= top) {  // the whole cluster
+    if (blockIdx.x == 0)
+      for (int i = tid; i < top; i += kSelectThreads) out[i] = i < n ? i : -1;
     return;
   }
+  score_chunks<T, D>(p, row, b, kvh, n, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (blockIdx.x > 0) return;
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const float* scores = p.scores + row * p.max_chunks;
   const bool shared = n <= kSelectShared;
   auto inner = [&](int i) { return i > 0 && i < n - 1; };
@@ -542,7 +543,6 @@ chunk_select_kernel(const SelectParams p) {
   int equal = 0;     // and how many of those that reach it are in
   if (ranked) {
     constexpr int LPC = ScoreLanes<D>::kLanes, CPS = ScoreLanes<D>::kChunks;
-    const int kvh = static_cast<int>(row % p.d.num_kv_heads);
     const int32_t* table = p.d.tables + b * p.d.table_stride;
     double wt[8];
     score_weights<T, D>(p, b, kvh, lane, wt);
@@ -635,11 +635,19 @@ static SparsePlan sparse_plan(const nib_sparse_decode_args& s) {
   if (n > by_len) n = by_len;
   if (n > 256) n = 256;
   pl.splits = static_cast<int>(n < 1 ? 1 : n);
-  // two score CTAs run on an SM: enough of them for two waves, or for all of a row's chunks at once
+  // score CTAs per row (a cluster): the fewest steps of a warp over all waves, the start and the
+  // selection counted as four
   const int64_t per_cta = kScoreWarps * kScoreUnroll * (a.head_dim == 64 ? 2 : 1);
-  const int64_t most = (pl.max_chunks + per_cta - 1) / per_cta;
-  pl.score_ctas = rows < 1 ? 1 : (4LL * sm_count() + rows - 1) / rows;
-  if (pl.score_ctas > most) pl.score_ctas = most;
+  const int64_t most = (pl.max_chunks + per_cta - 1) / per_cta, resident = static_cast<int64_t>(kScoreResident) * sm_count();
+  int64_t best = 0;
+  pl.score_ctas = 1;
+  for (int64_t c = 1; c <= 8 && c < 2 * most; c *= 2) {
+    const int64_t cost = (rows * c + resident - 1) / resident * ((most + c - 1) / c + 4);
+    if (best == 0 || cost < best) {
+      best = cost;
+      pl.score_ctas = c;
+    }
+  }
   pl.score_bytes = pl.max_chunks > s.top_chunks ? (rows * (pl.max_chunks * 12 + pl.score_ctas * kScoreWarps * 4) + 15) / 16 * 16 : 0;
   pl.partial_bytes = pl.splits > 1 ? nib::partial_bytes(a, pl.splits) : 0;
   return pl;
@@ -669,11 +677,8 @@ static int launch_sparse(const nib_sparse_decode_args& s, const SparsePlan& pl, 
     if ((1 << k) == sp.per) sp.per_shift = k;
   sp.max_chunks = pl.max_chunks;
   sp.selected = s.selected;
-  if (pl.score_bytes > 0) {
-    const dim3 grid(static_cast<unsigned>(pl.score_ctas), static_cast<unsigned>(rows));
-    launch_k(chunk_score_kernel<T, D>, grid, kScoreWarps * 32, 0, st, sp);
-  }
-  launch_k_pdl(pl.score_bytes > 0 || pdl_enabled(), chunk_select_kernel<T, D>, static_cast<unsigned>(rows), kSelectThreads, 0, st, sp);
+  launch_k_cluster(chunk_select_kernel<T, D>, dim3(static_cast<unsigned>(pl.score_ctas), static_cast<unsigned>(rows)),
+                   kSelectThreads, static_cast<unsigned>(pl.score_ctas), 0, st, sp);
   const int rc = launch_mma_mode<T, D, kDecodeSparse>(a, sp.d, rows, st, true);
   if (rc != NIB_OK || pl.splits == 1) return rc;
   return launch_combine_partials<T, D, kDecodeSparse>(a, sp.d, st);
