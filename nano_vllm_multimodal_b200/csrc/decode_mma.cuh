@@ -385,7 +385,7 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
   if (MODE == kDecodeSuffix && p.early) pdl_launch_dependents();  // runs next to it; waits for it at the end
   else pdl_enter();
 
-  const int kvh = static_cast<int>(blockIdx.x % p.num_kv_heads);
+  const int kvh = static_cast<int>(blockIdx.x) % p.num_kv_heads;
   const int split = blockIdx.y;
   int64_t b;          // the request whose table is read
   int64_t skip = 0;   // tokens before the range that the splits share
@@ -393,12 +393,12 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
   int64_t ctx = 0;    // kDecodeSparse: the request's length
   RowTile rt{};
   if constexpr (MODE == kDecodePrefix) {
-    rt = find_row_tile(p, blockIdx.x / p.num_kv_heads, 16, lane);
+    rt = find_row_tile(p, static_cast<int>(blockIdx.x) / p.num_kv_heads, 16, lane);
     if (rt.prefix == 0) return;  // no such tile, or nothing shared
     b = rt.leader;
     len = rt.prefix;
   } else {
-    b = blockIdx.x / p.num_kv_heads;
+    b = static_cast<int>(blockIdx.x) / p.num_kv_heads;
     len = clamped_len(p, b, threadIdx.x == 0 && split == 0);
     if constexpr (MODE == kDecodeSuffix) {
       skip = shared_prefix_of(p, b, len, lane);
@@ -406,36 +406,44 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     }
     if constexpr (MODE == kDecodeSparse) {
       ctx = len;
-      const int64_t chunks = (len + p.chunk - 1) / p.chunk;
-      len = (chunks < p.top ? chunks : p.top) * p.chunk;
+      const int chunks = static_cast<int>(len / p.chunk) + (len % p.chunk != 0);
+      len = static_cast<int64_t>(chunks < p.top ? chunks : p.top) * p.chunk;
     }
   }
-  // Split boundaries: the splits of a context shrink linearly toward the last one
-  // (split y gets a share s - y of s + (s-1) + ... + 1), and the grid's rows are
-  // dispatched in split order, so its final wave holds the smallest CTAs.
-  auto split_start = [&](int y) -> int64_t {
-    const int64_t sp = p.splits;
-    const int64_t before = y * sp - static_cast<int64_t>(y) * (y - 1) / 2;
-    return len * before / (sp * (sp + 1) / 2);
-  };
-  int64_t t_begin = skip + split_start(split);
-  int64_t t_end = skip + split_start(split + 1);
-  if constexpr (MODE == kDecodeSparse) {  // whole tiles: a chunk is a multiple of a tile
-    t_begin = t_begin / kMmaTile * kMmaTile;
-    t_end = t_end / kMmaTile * kMmaTile;
+  int64_t t_begin, t_end, tile0, n_tiles;
+  if constexpr (MODE == kDecodeFull) {
+    // Split boundaries: the splits of a context shrink linearly toward the last one
+    // (split y gets a share s - y of s + (s-1) + ... + 1), and the grid's rows are
+    // dispatched in split order, so its final wave holds the smallest CTAs.
+    auto split_start = [&](int y) -> int64_t {
+      const int64_t sp = p.splits;
+      const int64_t before = y * sp - static_cast<int64_t>(y) * (y - 1) / 2;
+      return len * before / (sp * (sp + 1) / 2);
+    };
+    t_begin = split_start(split);
+    t_end = split_start(split + 1);
+    tile0 = t_begin / kMmaTile;
+    n_tiles = t_end > t_begin ? (t_end + kMmaTile - 1) / kMmaTile - tile0 : 0;
+  } else {
+    // equal shares of whole tiles: one wave of CTAs is what these launches ask for
+    const int first = static_cast<int>(skip) / kMmaTile;
+    const int total = len > 0 ? static_cast<int>(skip + len + kMmaTile - 1) / kMmaTile - first : 0;
+    const int each = total / p.splits, more = total - each * p.splits;
+    tile0 = first + split * each + (split < more ? split : more);
+    n_tiles = each + (split < more ? 1 : 0);
+    t_begin = tile0 * kMmaTile > skip ? tile0 * kMmaTile : skip;
+    t_end = (tile0 + n_tiles) * kMmaTile < skip + len ? (tile0 + n_tiles) * kMmaTile : skip + len;
   }
-  const int64_t tile0 = t_begin / kMmaTile;
-  const int64_t n_tiles = t_end > t_begin ? (t_end + kMmaTile - 1) / kMmaTile - tile0 : 0;
   const int64_t n_mine = n_tiles > w ? (n_tiles - w + kMmaWarps - 1) / kMmaWarps : 0;  // warp-uniform
 
   const int r0 = lane >> 2, cq = (lane & 3) * 2;
   uint32_t qa[KS][4];
   if constexpr (MODE == kDecodePrefix) {
-    auto q_row = [&](int64_t r) -> const T* {
+    auto q_row = [&](int r) -> const T* {
       if (r >= (rt.end - rt.first) * p.group) return nullptr;
       return static_cast<const T*>(p.q) + (rt.first + r / p.group) * p.q_bs + (kvh * p.group + r % p.group) * p.q_hs;
     };
-    load_q_rows<T, D>(qa, q_row(rt.row0 + r0), q_row(rt.row0 + r0 + 8), lane);
+    load_q_rows<T, D>(qa, q_row(static_cast<int>(rt.row0) + r0), q_row(static_cast<int>(rt.row0) + r0 + 8), lane);
   } else {
     load_q_frags<T, D>(qa, static_cast<const T*>(p.q) + b * p.q_bs, p.q_hs, kvh * p.group, p.group, lane);
   }
@@ -463,12 +471,12 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
       if ((i & 31) == 0) {
         batch_blk = -1;
         if (i + lane < n_mine) {
-          int64_t t0 = (tile0 + w + (i + lane) * kMmaWarps) * kMmaTile;
+          int t0 = static_cast<int>(tile0 + w + (i + lane) * kMmaWarps) * kMmaTile;  // tokens stay below 2^31
           if constexpr (MODE == kDecodeSparse) {
-            const int64_t c = __ldg(list + t0 / p.chunk);
-            t0 = c < 0 ? ctx : c * p.chunk + t0 % p.chunk;
+            const int nth = t0 / p.chunk, c = __ldg(list + nth);
+            t0 = c < 0 ? static_cast<int>(ctx) : c * p.chunk + (t0 - nth * p.chunk);
           }
-          batch_t0 = static_cast<int>(t0);
+          batch_t0 = t0;
           if (MODE != kDecodeSparse || t0 < ctx) {  // a last chunk's empty tiles are left out
             batch_blk = __ldg(table + t0 / p.block_size);
             if (batch_blk < 0 || batch_blk >= p.num_blocks) {
@@ -590,10 +598,10 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     int64_t rb = b;
     int h = kvh * p.group + r;
     if constexpr (MODE == kDecodePrefix) {
-      const int64_t row = rt.row0 + r;
+      const int row = static_cast<int>(rt.row0) + r;
       if (row >= (rt.end - rt.first) * p.group) continue;
       rb = rt.first + row / p.group;
-      h = kvh * p.group + static_cast<int>(row % p.group);
+      h = kvh * p.group + row % p.group;
     }
     float M = -INFINITY;
 #pragma unroll
