@@ -50,6 +50,9 @@ constexpr int kMmaWarps = 4;
 constexpr int kMmaStages = 2;  // ring stages per warp: 3 CTAs (12 warps) per SM fit
 constexpr int kMmaTile = 16;   // tokens per tile
 
+// Contexts stay below this, so that token arithmetic a tile beyond them fits 32 bits.
+constexpr int64_t kMaxTokens = (int64_t{1} << 31) - 4096;
+
 // Which rows and tokens a CTA takes.
 enum DecodeMode : int {
   kDecodeFull = 0,    // a request's heads against all of its tokens

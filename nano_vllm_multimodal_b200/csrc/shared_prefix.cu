@@ -126,8 +126,8 @@ extern "C" int nib_shared_prefix_decode_attention(const nib_shared_prefix_args* 
   const int64_t group = a.num_heads / a.num_kv_heads;
   NIB_REQUIRE((a.batch * group + s->num_groups) * a.num_kv_heads <= 0x7fffffffLL && a.batch * a.num_heads <= 0x7fffffffLL,
               "shared_prefix_decode_attention: batch too large");
-  NIB_REQUIRE(a.max_blocks_per_seq * a.block_size < (int64_t{1} << 31),
-              "shared_prefix_decode_attention: block table covers 2^31 tokens or more");
+  NIB_REQUIRE(a.max_blocks_per_seq * a.block_size < kMaxTokens,
+              "shared_prefix_decode_attention: block table covers too many tokens (2^31 - 4096)");
   NIB_SUPPORT(aligned16(a.q) && a.q_batch_stride % 8 == 0 && a.q_head_stride % 8 == 0,
               "shared_prefix_decode_attention: q must be 16-byte aligned with strides of multiples of 8 elements");
   NIB_SUPPORT(decode_mma_eligible(a), "shared_prefix_decode_attention: needs bf16/f16, head_dim 64 or 128, at most 16 q "

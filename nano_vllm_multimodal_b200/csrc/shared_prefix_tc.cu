@@ -77,10 +77,24 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   unsigned char* dsm = dsm_raw + (base - raw);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 
+  pdl_enter();
+
+  const int kvh = static_cast<int>(blockIdx.x) % p.num_kv_heads;
+  const int split = blockIdx.y;
+  const RowTile rt = find_row_tile(p, static_cast<int>(blockIdx.x) / p.num_kv_heads, 2 * kPtRows, lane);
+  if (rt.prefix == 0) return;
+  const int group_rows = static_cast<int>(rt.end - rt.first) * p.group, row0 = static_cast<int>(rt.row0);
+  const int prefix = static_cast<int>(rt.prefix);  // a table covers less than 2^31 tokens
+  const int rows = group_rows - row0 < 2 * kPtRows ? group_rows - row0 : 2 * kPtRows;
+  const bool both = rows > kPtRows;  // each stream has rows of its own
+  const int tiles = static_cast<int>((rt.prefix + kPtTile - 1) / kPtTile);
+  const int each = tiles / p.splits, more = tiles - each * p.splits;
+  const int tile0 = split * each + (split < more ? split : more), n = each + (split < more ? 1 : 0);
+  const int32_t* table = p.tables + rt.leader * p.table_stride;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPtSlots; ++i) {
       mbar_init(&bars.full[i], 1);
-      mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.empty[i], both ? 2 : 1);  // the streams that use a tile
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
@@ -91,19 +105,6 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     bars.abort = 0;
     fence_mbar_init();
   }
-  pdl_enter();
-
-  const int kvh = static_cast<int>(blockIdx.x % p.num_kv_heads);
-  const int split = blockIdx.y;
-  const RowTile rt = find_row_tile(p, blockIdx.x / p.num_kv_heads, 2 * kPtRows, lane);
-  if (rt.prefix == 0) return;
-  const int64_t group_rows = (rt.end - rt.first) * p.group;
-  const int rows = static_cast<int>(group_rows - rt.row0 < 2 * kPtRows ? group_rows - rt.row0 : 2 * kPtRows);
-  const bool both = rows > kPtRows;  // each stream has rows of its own
-  const int64_t tiles = (rt.prefix + kPtTile - 1) / kPtTile;
-  const int64_t tile0 = tiles * split / p.splits;
-  const int n = static_cast<int>(tiles * (split + 1) / p.splits - tile0);
-  const int32_t* table = p.tables + rt.leader * p.table_stride;
   // stream s: its number of tiles and its i-th one; the ring's load number of tile t's K and V
   // (in the order in which the MMAs want them; a number that has no tile is left out, and no
   // later one comes round to its slot)
@@ -121,7 +122,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       const int r = e / kVecs, c = e % kVecs;
       uint4 v = zero_vec();
       if (r < rows) {
-        const int64_t row = rt.row0 + r;
+        const int row = row0 + r;
         v = ld_vec(static_cast<const T*>(p.q) + (rt.first + row / p.group) * p.q_bs +
                    (kvh * p.group + row % p.group) * p.q_hs + c * 8);
         if (flip) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
@@ -161,10 +162,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       if (t >= n) continue;
       const int slot = num % kPtSlots;
-      const int64_t tok = (tile0 + t) * kPtTile;
-      const int64_t at = tok + lane * pp.box;
+      const int tok = (tile0 + t) * kPtTile, at = tok + lane * pp.box;
       int page = -1;
-      if (lane < boxes && at < rt.prefix) {
+      if (lane < boxes && at < prefix) {
         page = __ldg(table + at / p.block_size);
         if (page < 0 || page >= p.num_blocks) {
           page = -1;
@@ -172,7 +172,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
       }
       const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
-      const bool whole = __popc(have) == boxes && tok + kPtTile <= rt.prefix;
+      const bool whole = __popc(have) == boxes && tok + kPtTile <= prefix;
       bool ok = true;
       if (num >= kPtSlots) ok = pt_wait(bars, &bars.empty[slot], static_cast<uint32_t>((num / kPtSlots - 1) & 1));
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -182,7 +182,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       __syncwarp();
       if (page >= 0) {
         const uint32_t dst = ring + slot * L::kSlot + lane * pp.box * 128;
-        const int off = static_cast<int>(at % p.block_size);
+        const int off = at % p.block_size;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
           tma_load_5d(dst + c * (kPtTile * 128), is_v ? &vmap : &kmap, 0, c, kvh, off, page, bar);
@@ -193,7 +193,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         if (!__all_sync(0xffffffffu, ok)) break;
         for (int e = lane; e < kPtTile * (D / 8); e += 32) {
           const int row = e % kPtTile, c = e / kPtTile;
-          if (tok + row >= rt.prefix || !((have >> (row / pp.box)) & 1u))
+          if (tok + row >= prefix || !((have >> (row / pp.box)) & 1u))
             *reinterpret_cast<uint4*>(dsm + 2 * L::kQ + slot * L::kSlot + (c / 8) * (kPtTile * 128) + row * 128 + (c % 8) * 16) = zero_vec();
         }
         fence_proxy_async();
@@ -201,48 +201,42 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         if (lane == 0) mbar_arrive(&bars.full[slot]);
       }
     }
-  } else if (w == 1) {
-    // ---------------------------------------------------------------- MMAs
+  } else if (w <= 2) {
+    // ---------------------------------------------------------------- MMAs, a warp per stream
     if (lane == 0) {
       constexpr uint32_t kIdS = mma_idesc(kBf16, kPtRows, kPtTile, false);
       constexpr uint32_t kIdO = mma_idesc(kBf16, kPtRows, D, true);
+      const int s = w - 1, mine = steps(s);
+      const uint32_t q = base + (both ? s * L::kQ : 0u), ts = tmem + s * 128, to = tmem + 256 + s * 128;
       auto full = [&](int num) { return pt_wait(bars, &bars.full[num % kPtSlots], static_cast<uint32_t>((num / kPtSlots) & 1)); };
-      auto scores = [&](int s, int i) -> bool {  // S_s = Q_s K^T of the stream's i-th tile
+      auto scores = [&](int i) -> bool {  // S = Q K^T of the stream's i-th tile
         const int num = k_load(tile_of(s, i));
         if (!full(num)) return false;
         tc_fence_after();
-        const uint32_t q = base + (both ? s * L::kQ : 0u), k = ring + (num % kPtSlots) * L::kSlot;
+        const uint32_t k = ring + (num % kPtSlots) * L::kSlot;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t at = (kk / 4) * (kPtRows * 128) + (kk % 4) * 32;
-          tc_mma_ss(tmem + s * 128, smem_desc(q + at, 16, 1024), smem_desc(k + at, 16, 1024), kIdS, kk > 0);
+          tc_mma_ss(ts, smem_desc(q + at, 16, 1024), smem_desc(k + at, 16, 1024), kIdS, kk > 0);
         }
         tc_commit(&bars.s_full[s]);
-        if (!both || s == 1) tc_commit(&bars.empty[num % kPtSlots]);
+        tc_commit(&bars.empty[num % kPtSlots]);
         return true;
       };
-      bool ok = true;
-      for (int s = 0; s < 2 && ok; ++s)
-        if (steps(s) > 0) ok = scores(s, 0);
-      for (int i = 0; ok && i < steps(0); ++i) {
-        for (int s = 0; s < 2 && ok; ++s) {
-          if (i >= steps(s)) continue;
-          const int num = v_load(tile_of(s, i));
-          ok = pt_wait(bars, &bars.p_full[s], static_cast<uint32_t>(i & 1)) && full(num);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t v = ring + (num % kPtSlots) * L::kSlot;
+      bool ok = mine == 0 || scores(0);
+      for (int i = 0; ok && i < mine; ++i) {
+        const int num = v_load(tile_of(s, i));
+        ok = full(num) && pt_wait(bars, &bars.p_full[s], static_cast<uint32_t>(i & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v = ring + (num % kPtSlots) * L::kSlot;
 #pragma unroll
-          for (int kk = 0; kk < kPtTile / 16; ++kk)
-            tc_mma_ts(tmem + 256 + s * 128, tmem + s * 128 + kk * 8, smem_desc(v + kk * 2048, kPtTile * 128, 1024), kIdO,
-                      i > 0 || kk > 0);
-          tc_commit(&bars.o_done[s]);
-          if (!both || s == 1) tc_commit(&bars.empty[num % kPtSlots]);
-          if (i + 1 < steps(s)) {
-            // the next scores overwrite P: only after the product that reads it
-            ok = pt_wait(bars, &bars.o_done[s], static_cast<uint32_t>(i & 1)) && scores(s, i + 1);
-          }
-        }
+        for (int kk = 0; kk < kPtTile / 16; ++kk)
+          tc_mma_ts(to, ts + kk * 8, smem_desc(v + kk * 2048, kPtTile * 128, 1024), kIdO, i > 0 || kk > 0);
+        tc_commit(&bars.o_done[s]);
+        tc_commit(&bars.empty[num % kPtSlots]);
+        // the next scores overwrite P: only after the product that reads it
+        if (i + 1 < mine) ok = pt_wait(bars, &bars.o_done[s], static_cast<uint32_t>(i & 1)) && scores(i + 1);
       }
     }
     __syncwarp();
@@ -257,10 +251,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int i = 0; i < mine; ++i) {
-      const int64_t tok = (tile0 + tile_of(s, i)) * kPtTile;
-      const int64_t at = tok + lane * pp.box;
+      const int tok = (tile0 + tile_of(s, i)) * kPtTile, at = tok + lane * pp.box;
       bool here = false;
-      if (lane < boxes && at < rt.prefix) {
+      if (lane < boxes && at < prefix) {
         const int page = __ldg(table + at / p.block_size);
         here = page >= 0 && page < p.num_blocks;
       }
@@ -269,9 +262,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       if (!ok) break;
       tc_fence_after();
       // scores behind the prefix or without a page: -inf (warp-uniform, rare)
-      const bool whole = __popc(have) == boxes && tok + kPtTile <= rt.prefix;
+      const bool whole = __popc(have) == boxes && tok + kPtTile <= prefix;
       auto mask = [&](uint32_t* x, int c) {
-        const int64_t left = rt.prefix - tok - c * 32;
+        const int left = prefix - tok - c * 32;
         uint32_t bits = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;  // tokens before the prefix's end
         if (!((have >> (c * 32 / pp.box)) & 1u)) bits &= 0xffff0000u;
         if (!((have >> ((c * 32 + 16) / pp.box)) & 1u)) bits &= 0x0000ffffu;
@@ -279,21 +272,21 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         for (int e = 0; e < 32; ++e)
           if (!((bits >> e) & 1u)) x[e] = 0xff800000u;
       };
-      // the row is read twice, 32 columns at a time: once for its maximum, once for P
-      float mx = -INFINITY;
+      uint32_t x[kPtTile];
 #pragma unroll
-      for (int c = 0; c < kPtTile / 32; c += 2) {
-        uint32_t x[64];
-        tmem_ld32(ts + c * 32, x);
-        tmem_ld32(ts + c * 32 + 32, x + 32);
-        tmem_wait_ld();
-        if (!whole) {
-          mask(x, c);
-          mask(x + 32, c + 1);
-        }
+      for (int c = 0; c < kPtTile / 32; ++c) tmem_ld32(ts + c * 32, x + c * 32);
+      tmem_wait_ld();
+      if (!whole) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(x[e]));
+        for (int c = 0; c < kPtTile / 32; ++c) mask(x + c * 32, c);
       }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < kPtTile; e += 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], __uint_as_float(x[e + k]), __uint_as_float(x[e + 4 + k]));
+      }
+      float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
       mx *= qs;
       if (i == 0) {
         m = mx;
@@ -307,33 +300,33 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         m = up ? mx : m;
         l *= f;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(to + c * 32, o);
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(to + c * 16, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st32(to + c * 32, o);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st16(to + c * 16, o);
         }
       }
       const float sub = m == -INFINITY ? 0.f : m;  // a row of nothing but masked tokens: all P are 0
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t qs2 = pair2(qs, qs), sub2 = pair2(-sub, -sub);
+      uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < kPtTile / 32; ++c) {
-        uint32_t x[32], pk[16];
-        tmem_ld32(ts + c * 32, x);
-        tmem_wait_ld();
-        if (!whole) mask(x, c);
+      for (int c = 0; c < kPtTile / 64; ++c) {
+        uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float a = ex2_fast(fmaf(__uint_as_float(x[2 * e]), qs, -sub));
-          const float b = ex2_fast(fmaf(__uint_as_float(x[2 * e + 1]), qs, -sub));
-          part[e & 3] += a + b;
+        for (int e = 0; e < 32; ++e) {
+          const int k = c * 64 + 2 * e;
+          const float2 y = unpair2(fma2(pair2(x[k], x[k + 1]), qs2, sub2));
+          const float a = ex2_fast(y.x), b = ex2_fast(y.y);
+          part[e & 1] = add2(part[e & 1], pair2(a, b));
           pk[e] = pack2<T>(a, b);
         }
-        tmem_st16(ts + c * 16, pk);  // over columns that have been read
+        tmem_st32(ts + c * 32, pk);
       }
-      l += (part[0] + part[1]) + (part[2] + part[3]);
+      const float2 sum = unpair2(add2(part[0], part[1]));
+      l += sum.x + sum.y;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bars.p_full[s]);
@@ -360,7 +353,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
     }
-    const int64_t row = rt.row0 + (both ? s * kPtRows : 0) + r;
+    const int row = row0 + (both ? s * kPtRows : 0) + r;
     const bool writes = ok && (both || s == 0) && row < group_rows;
     float fa = 1.f, fb = 0.f;
     if (!both && s == 0) {
@@ -372,7 +365,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     }
     if (both || s == 0) {
       const int64_t b = rt.first + (row < group_rows ? row / p.group : 0);
-      const int h = kvh * p.group + static_cast<int>(row % p.group);
+      const int h = kvh * p.group + row % p.group;
       const int64_t place = (b * p.num_heads + h) * p.slots + p.slot0 + split;
       float* ws = p.ws + place * D;
 #pragma unroll

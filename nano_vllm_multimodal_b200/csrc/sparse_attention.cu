@@ -716,7 +716,7 @@ extern "C" int nib_paged_key_bounds(int dtype, const void* key_cache, int64_t ca
   if (batch == 0 || max_new_tokens == 0 || max_blocks_per_seq == 0) return NIB_OK;
   NIB_REQUIRE(key_cache && block_tables && start_lens && context_lens && bounds, "paged_key_bounds: null pointer");
   NIB_REQUIRE(block_size < (int64_t{1} << 31) && max_blocks_per_seq * block_size < (int64_t{1} << 31),
-              "paged_key_bounds: block table covers 2^31 tokens or more");
+              "paged_key_bounds: block table covers too many tokens (2^31 - 4096)");
   NIB_SUPPORT(batch <= 65535 && num_kv_heads <= 4096, "paged_key_bounds: at most 65535 sequences and 4096 kv heads");
   NIB_SUPPORT(aligned16(key_cache) && aligned16(bounds) && cache_block_stride % 8 == 0 && cache_slot_stride % 8 == 0 &&
                   cache_head_stride % 8 == 0 && bounds_block_stride % 8 == 0 && bounds_head_stride % 8 == 0,
@@ -770,8 +770,8 @@ extern "C" int nib_sparse_decode_attention(const nib_sparse_decode_args* s, void
   NIB_REQUIRE(a.q && a.key_cache && a.value_cache && a.block_tables && a.context_lens && a.out && s->bounds && s->selected,
               "sparse_decode_attention: null pointer");
   NIB_SUPPORT(a.batch * a.num_kv_heads <= 65535, "sparse_decode_attention: at most 65535 (request, kv head) pairs");
-  NIB_REQUIRE(a.max_blocks_per_seq * a.block_size < (int64_t{1} << 31),
-              "sparse_decode_attention: block table covers 2^31 tokens or more");
+  NIB_REQUIRE(a.max_blocks_per_seq * a.block_size < kMaxTokens,
+              "sparse_decode_attention: block table covers too many tokens (2^31 - 4096)");
   NIB_SUPPORT(aligned16(a.q) && a.q_batch_stride % 8 == 0 && a.q_head_stride % 8 == 0 && aligned16(s->bounds) &&
                   s->bounds_block_stride % 8 == 0 && s->bounds_head_stride % 8 == 0,
               "sparse_decode_attention: q and bounds must be 16-byte aligned with strides of multiples of 8 elements");
