@@ -43,6 +43,7 @@ struct PtSmem {
 struct PtBars {
   uint64_t full[kPtSlots], empty[kPtSlots];
   uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t turn[2][4];  // whose exponentials are next, per pair of warps on a scheduler
   uint64_t landed;  // copies of a tile that is mended before it counts as full
   uint32_t tmem;
   int abort;
@@ -100,6 +101,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_full[i], 128);
       mbar_init(&bars.o_done[i], 1);
+      for (int k = 0; k < 4; ++k) mbar_init(&bars.turn[i][k], 1);
     }
     mbar_init(&bars.landed, 1);
     bars.abort = 0;
@@ -203,43 +205,57 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     }
   } else if (w <= 2) {
     // ---------------------------------------------------------------- MMAs, a warp per stream
-    if (lane == 0) {
-      constexpr uint32_t kIdS = mma_idesc(kBf16, kPtRows, kPtTile, false);
-      constexpr uint32_t kIdO = mma_idesc(kBf16, kPtRows, D, true);
-      const int s = w - 1, mine = steps(s);
-      const uint32_t q = base + (both ? s * L::kQ : 0u), ts = tmem + s * 128, to = tmem + 256 + s * 128;
-      auto full = [&](int num) { return pt_wait(bars, &bars.full[num % kPtSlots], static_cast<uint32_t>((num / kPtSlots) & 1)); };
-      auto scores = [&](int i) -> bool {  // S = Q K^T of the stream's i-th tile
-        const int num = k_load(tile_of(s, i));
-        if (!full(num)) return false;
-        tc_fence_after();
-        const uint32_t k = ring + (num % kPtSlots) * L::kSlot;
+    // The whole warp runs the loop and waits; one lane issues. Operand addresses change in the
+    // descriptors' low words only.
+    constexpr uint32_t kIdS = mma_idesc(kBf16, kPtRows, kPtTile, false);
+    constexpr uint32_t kIdO = mma_idesc(kBf16, kPtRows, D, true);
+    const int s = w - 1, mine = steps(s);
+    const uint32_t ts = tmem + s * 128, to = tmem + 256 + s * 128;
+    const uint64_t q_desc = smem_desc(base + (both ? s * L::kQ : 0u), 16, 1024);
+    const uint64_t k_desc = smem_desc(ring, 16, 1024), v_desc = smem_desc(ring, kPtTile * 128, 1024);
+    const bool leader = elect_one();
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, pt_wait(bars, bar, parity)) != 0; };
+    auto scores = [&](int num) {  // S = Q K^T, K by the ring's load `num`
+      tc_fence_after();
+      const int slot = num % kPtSlots;
+      const uint64_t k = k_desc + slot * (L::kSlot >> 4);
+      if (leader) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t at = (kk / 4) * (kPtRows * 128) + (kk % 4) * 32;
-          tc_mma_ss(ts, smem_desc(q + at, 16, 1024), smem_desc(k + at, 16, 1024), kIdS, kk > 0);
+          constexpr uint32_t kHalf = kPtRows * 128;
+          const uint32_t at = ((kk / 4) * kHalf + (kk % 4) * 32) >> 4;
+          tc_mma_ss(ts, q_desc + at, k + at, kIdS, kk > 0);
         }
         tc_commit(&bars.s_full[s]);
-        tc_commit(&bars.empty[num % kPtSlots]);
-        return true;
-      };
-      bool ok = mine == 0 || scores(0);
-      for (int i = 0; ok && i < mine; ++i) {
-        const int num = v_load(tile_of(s, i));
-        ok = full(num) && pt_wait(bars, &bars.p_full[s], static_cast<uint32_t>(i & 1));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t v = ring + (num % kPtSlots) * L::kSlot;
+        tc_commit(&bars.empty[slot]);
+      }
+    };
+    bool ok = true;
+    if (mine > 0) {
+      const int num = k_load(tile_of(s, 0));
+      ok = wait_all(&bars.full[num % kPtSlots], static_cast<uint32_t>((num / kPtSlots) & 1));
+      if (ok) scores(num);
+    }
+    for (int i = 0; ok && i < mine; ++i) {
+      const int num = v_load(tile_of(s, i)), slot = num % kPtSlots;
+      const int next = i + 1 < mine ? k_load(tile_of(s, i + 1)) : -1;
+      ok = wait_all(&bars.full[slot], static_cast<uint32_t>((num / kPtSlots) & 1)) && wait_all(&bars.p_full[s], static_cast<uint32_t>(i & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t v = v_desc + slot * (L::kSlot >> 4);
+      if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < kPtTile / 16; ++kk)
-          tc_mma_ts(to, ts + kk * 8, smem_desc(v + kk * 2048, kPtTile * 128, 1024), kIdO, i > 0 || kk > 0);
+        for (int kk = 0; kk < kPtTile / 16; ++kk) tc_mma_ts(to, ts + kk * 8, v + kk * (2048 >> 4), kIdO, i > 0 || kk > 0);
         tc_commit(&bars.o_done[s]);
-        tc_commit(&bars.empty[num % kPtSlots]);
+        tc_commit(&bars.empty[slot]);
+      }
+      if (next >= 0) {
         // the next scores overwrite P: only after the product that reads it
-        if (i + 1 < mine) ok = pt_wait(bars, &bars.o_done[s], static_cast<uint32_t>(i & 1)) && scores(i + 1);
+        ok = wait_all(&bars.full[next % kPtSlots], static_cast<uint32_t>((next / kPtSlots) & 1)) &&
+             wait_all(&bars.o_done[s], static_cast<uint32_t>(i & 1));
+        if (ok) scores(next);
       }
     }
-    __syncwarp();
   } else if (w >= 4) {
     // ---------------------------------------------------------------- softmax
     const int s = (w - 4) >> 2;
@@ -310,6 +326,11 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
       }
       const float sub = m == -INFINITY ? 0.f : m;  // a row of nothing but masked tokens: all P are 0
+      // the streams take turns: stream 0's step i, stream 1's step i, stream 0's step i + 1, ...
+      if (s == 1 || i > 0) {
+        ok = __all_sync(0xffffffffu, pt_wait(bars, &bars.turn[s][w & 3], static_cast<uint32_t>((s == 1 ? i : i - 1) & 1)));
+        if (!ok) break;
+      }
       const uint64_t qs2 = pair2(qs, qs), sub2 = pair2(-sub, -sub);
       uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
@@ -325,6 +346,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
         tmem_st32(ts + c * 32, pk);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.turn[1 - s][w & 3]);
       const float2 sum = unpair2(add2(part[0], part[1]));
       l += sum.x + sum.y;
       tmem_wait_st();
