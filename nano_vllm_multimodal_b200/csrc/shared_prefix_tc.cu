@@ -117,21 +117,25 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
   // ---- Q rows into shared memory (swizzled 128-byte rows, one 16 KB region per 64 channels)
   {
-    constexpr int kVecs = D / 8;
-    const bool flip = p.qscale < 0.f;  // the maximum is taken before the scale
-    const int have = both ? 2 * kPtRows : kPtRows;
-    for (int e = threadIdx.x; e < have * kVecs; e += kPtThreads) {
-      const int r = e / kVecs, c = e % kVecs;
-      uint4 v = zero_vec();
-      if (r < rows) {
-        const int row = row0 + r;
-        v = ld_vec(static_cast<const T*>(p.q) + (rt.first + row / p.group) * p.q_bs +
-                   (kvh * p.group + row % p.group) * p.q_hs + c * 8);
-        if (flip) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+    constexpr int kVecs = D / 8, kTake = 2 * kPtRows * kVecs / kPtThreads + 1;  // vectors per thread
+    const uint32_t flip = p.qscale < 0.f ? 0x80008000u : 0u;  // the maximum is taken before the scale
+    const int have = (both ? 2 * kPtRows : kPtRows) * kVecs;
+    uint4 v[kTake];  // all of a thread's loads in flight
+#pragma unroll
+    for (int k = 0; k < kTake; ++k) {
+      const int e = threadIdx.x + k * kPtThreads, r = e / kVecs, row = row0 + r;
+      v[k] = zero_vec();
+      if (e < have && r < rows) {
+        const int request = row / p.group;
+        v[k] = ld_vec(static_cast<const T*>(p.q) + (rt.first + request) * p.q_bs +
+                      (kvh * p.group + row - request * p.group) * p.q_hs + e % kVecs * 8);
       }
-      const int in = r % kPtRows;
+    }
+#pragma unroll
+    for (int k = 0; k < kTake; ++k) {
+      const int e = threadIdx.x + k * kPtThreads, r = e / kVecs, c = e % kVecs, in = r % kPtRows;
       const uint32_t at = (r / kPtRows) * L::kQ + (c / 8) * (kPtRows * 128) + in * 128 + (((c % 8) ^ (in & 7)) << 4);
-      *reinterpret_cast<uint4*>(dsm + at) = v;
+      if (e < have) *reinterpret_cast<uint4*>(dsm + at) = make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip);
     }
     fence_proxy_async();
   }
@@ -387,26 +391,33 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       m = top;
     }
     if (both || s == 0) {
-      const int64_t b = rt.first + (row < group_rows ? row / p.group : 0);
-      const int h = kvh * p.group + row % p.group;
-      const int64_t place = (b * p.num_heads + h) * p.slots + p.slot0 + split;
-      float* ws = p.ws + place * D;
+      // 32 columns of the warp's rows at a time, through the stream's Q (its products have
+      // ended), so that eight lanes write 128 bytes of a row
+      const int64_t request = rt.first + (row < group_rows ? row / p.group : 0);
+      const int64_t place = writes ? (request * p.num_heads + kvh * p.group + row % p.group) * p.slots + p.slot0 + split : -1;
+      float4* turn = reinterpret_cast<float4*>(dsm + s * L::kQ) + (w & 3) * 256;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(to + c * 32, o);
         tmem_wait_ld();
-        if (writes) {
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float v[4];
+        for (int e = 0; e < 32; e += 4) {
+          float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[k] = mine > 0 ? __uint_as_float(o[e + k]) : 0.f;
-              if (!both) v[k] = v[k] * fa + meet[(2 + c * 32 + e + k) * kPtRows + r] * fb;
-            }
-            *reinterpret_cast<float4*>(ws + c * 32 + e) = make_float4(v[0], v[1], v[2], v[3]);
+          for (int k = 0; k < 4; ++k) {
+            v[k] = mine > 0 ? __uint_as_float(o[e + k]) : 0.f;
+            if (!both) v[k] = v[k] * fa + meet[(2 + c * 32 + e + k) * kPtRows + r] * fb;
           }
+          turn[lane * 8 + ((e / 4) ^ (lane & 7))] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int from = k * 4 + lane / 8;
+          const int64_t at = __shfl_sync(0xffffffffu, place, from);
+          if (at >= 0) *reinterpret_cast<float4*>(p.ws + at * D + c * 32 + lane % 8 * 4) = turn[from * 8 + ((lane % 8) ^ (from & 7))];
         }
       }
       if (writes) p.ml[place] = make_float2(m, l);
