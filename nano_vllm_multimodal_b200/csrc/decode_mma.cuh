@@ -638,60 +638,88 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
 }
 
 
-// out[b, h] from the partials of (b, h): one CTA, its warps by turns over the partials, so that
-// two round trips to memory are all it takes (maxima and sums, then outputs). MODE
-// kDecodeSuffix: the first slot0 partials are the prefix's, which only a request that shares
-// one has.
-constexpr int kCombineWarps = 4;
+// out[b, h] from the partials of (b, h). MODE kDecodeSuffix: the first slot0 partials are the
+// prefix's, which only a request that shares one has. WPR warps take a row's partials by turns; a
+// warp's first eight outputs are requested together with the maxima and sums, before it is known
+// which of them count: one round trip to memory is most of this kernel's time. (Four warps a row
+// where rows are few, one where they fill the SMs: 4,096 rows of ten partials, 13.2 us with four.)
+constexpr int kCombineWarps = 4, kCombineBatch = 8;
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, int WPR>
 __global__ void __launch_bounds__(kCombineWarps * 32)
 combine_partials_kernel(const MmaDecodeParams p) {
   pdl_enter();
   constexpr int E = D / 32;  // channels per lane
-  __shared__ float red[kCombineWarps][D];
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  __shared__ float red[WPR > 1 ? kCombineWarps : 1][D];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t bh = blockIdx.x;
-  const int64_t b = bh / p.num_heads;
-  const int h = static_cast<int>(bh % p.num_heads);
+  const int row = static_cast<int>(blockIdx.x) * (kCombineWarps / WPR) + w / WPR, part = w % WPR;
+  if (row >= static_cast<int>(p.batch) * p.num_heads) return;  // WPR = 1 alone
+  const int b = row / p.num_heads, h = row - b * p.num_heads;
+  const float2* ml = p.ml + static_cast<int64_t>(row) * p.slots;
+  const Vec* ws = reinterpret_cast<const Vec*>(p.ws + static_cast<int64_t>(row) * p.slots * D) + lane;
+  Vec v[kCombineBatch];
+#pragma unroll
+  for (int k = 0; k < kCombineBatch; ++k)
+    if (part + k * WPR < p.slots) v[k] = ws[static_cast<int64_t>(part + k * WPR) * 32];
+  const float2 first = lane < p.slots ? ml[lane] : make_float2(-INFINITY, 0.f);
   int s0 = 0;
   if constexpr (MODE == kDecodeSuffix) {
     if (shared_prefix_of(p, b, clamped_len(p, b, false), lane) == 0) s0 = p.slot0;
   }
-  const float2* ml = p.ml + bh * p.slots;
-  const float* ws = p.ws + bh * p.slots * D + lane * E;
-  float M = -INFINITY;
-  for (int s = s0 + lane; s < p.slots; s += 32) M = fmaxf(M, ml[s].x);
+  float M = lane >= s0 ? first.x : -INFINITY;
+  for (int s = 32 + lane; s < p.slots; s += 32)
+    if (s >= s0) M = fmaxf(M, ml[s].x);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (M != -INFINITY) {
-    for (int s = s0 + lane; s < p.slots; s += 32) L += ml[s].y * ex2_fast(ml[s].x - M);
+    // a split without tokens has no output and the weight 0
+    auto weight = [&](float2 x, int s) { return s >= s0 && x.x != -INFINITY ? ex2_fast(x.x - M) : 0.f; };
+    const float f = weight(first, lane);
+    L = f > 0.f ? first.y * f : 0.f;
+    for (int s = 32 + lane; s < p.slots; s += 32) {
+      const float2 x = ml[s];
+      const float g = weight(x, s);
+      if (g > 0.f) L += x.y * g;
+    }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-#pragma unroll 4
-    for (int s = s0 + w; s < p.slots; s += kCombineWarps) {
-      const float m = ml[s].x;
-      if (m == -INFINITY) continue;  // a split without tokens: its output is not written
-      const float f = ex2_fast(m - M);
+    auto add = [&](const Vec& x, float g) {
+      const float* xs = reinterpret_cast<const float*>(&x);
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(ws + static_cast<int64_t>(s) * D + e);
-        acc[e] += v.x * f;
-        acc[e + 1] += v.y * f;
-      }
+      for (int e = 0; e < E; ++e) acc[e] += xs[e] * g;
+    };
+#pragma unroll
+    for (int k = 0; k < kCombineBatch; ++k) {
+      const int s = part + k * WPR;  // below 32
+      const float g = __shfl_sync(0xffffffffu, f, s);
+      if (s < p.slots && g > 0.f) add(v[k], g);
+    }
+    for (int s = part + kCombineBatch * WPR; s < p.slots; s += WPR) {
+      const float g = weight(ml[s], s);
+      if (g > 0.f) add(ws[static_cast<int64_t>(s) * 32], g);
     }
   }
+  T* out = static_cast<T*>(p.out) + b * p.o_bs + h * p.o_hs;
+  if constexpr (WPR == 1) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) red[w][lane * E + e] = acc[e];
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += kCombineWarps * 32) {
-    float A = 0.f;
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<typename Vec2<T>::type*>(out + lane * E + e) =
+          Vec2<T>::make(L > 0.f ? acc[e] / L : 0.f, L > 0.f ? acc[e + 1] / L : 0.f);
+  } else {
 #pragma unroll
-    for (int ww = 0; ww < kCombineWarps; ++ww) A += red[ww][d];
-    static_cast<T*>(p.out)[b * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
+    for (int e = 0; e < E; ++e) red[w][lane * E + e] = acc[e];
+    __syncthreads();
+    static_assert(WPR == kCombineWarps, "a CTA per row");
+    for (int d = threadIdx.x; d < D; d += kCombineWarps * 32) {
+      float A = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < kCombineWarps; ++ww) A += red[ww][d];
+      out[d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
+    }
   }
 }
 
@@ -707,7 +735,15 @@ inline void place_partials(MmaDecodeParams& p, const nib_decode_attention_args& 
 
 template <typename T, int D, int MODE>
 int launch_combine_partials(const nib_decode_attention_args& a, const MmaDecodeParams& p, cudaStream_t st) {
-  launch_k_after(combine_partials_kernel<T, D, MODE>, static_cast<unsigned>(a.batch * a.num_heads), kCombineWarps * 32, 0, st, p);
+  static_assert(kCombineBatch * kCombineWarps <= 32, "a batch's weights lie in one warp");
+  const int64_t rows = a.batch * a.num_heads;
+  // one warp a row once that gives every SM 16 warps
+  if (rows >= 16LL * sm_count()) {
+    const unsigned grid = static_cast<unsigned>((rows + kCombineWarps - 1) / kCombineWarps);
+    launch_k_after(combine_partials_kernel<T, D, MODE, 1>, grid, kCombineWarps * 32, 0, st, p);
+  } else {
+    launch_k_after(combine_partials_kernel<T, D, MODE, kCombineWarps>, static_cast<unsigned>(rows), kCombineWarps * 32, 0, st, p);
+  }
   return launch_status("decode_attention (combine)");
 }
 
