@@ -57,7 +57,8 @@ constexpr int64_t kMaxTokens = (int64_t{1} << 31) - 4096;
 enum DecodeMode : int {
   kDecodeFull = 0,    // a request's heads against all of its tokens
   kDecodeSuffix = 1,  // a request's heads against its tokens behind the prefix that its group shares
-  kDecodePrefix = 2,  // 16 rows (request, head) of a group against the prefix that they share
+  kDecodeShared = 2,  // one launch: 16 rows (request, head) of a group against the prefix that they
+                      // share (the first prefix_ctas CTAs), and kDecodeSuffix's work
   kDecodeSparse = 3   // a request's heads against the chunks selected for them
 };
 
@@ -79,7 +80,8 @@ struct MmaDecodeParams {
   int slots, slot0;  // partials per (request, head), and this launch's first
   bool early;  // kDecodeSuffix: launched behind the prefix kernel, of whose results it reads none
   unsigned int* status;
-  // kDecodeSuffix, kDecodePrefix
+  // kDecodeSuffix, kDecodeShared
+  int prefix_ctas, prefix_splits;
   int64_t batch;
   const int32_t* group_offsets;  // [num_groups + 1]
   const int32_t* prefix_lens;    // [num_groups]
@@ -388,22 +390,30 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
   if (MODE == kDecodeSuffix && p.early) pdl_launch_dependents();  // runs next to it; waits for it at the end
   else pdl_enter();
 
-  const int kvh = static_cast<int>(blockIdx.x) % p.num_kv_heads;
-  const int split = blockIdx.y;
+  // kDecodeShared: a 1-D grid; else (rows x kv heads, splits)
+  const bool is_prefix = MODE == kDecodeShared && static_cast<int>(blockIdx.x) < p.prefix_ctas;
+  const int splits = is_prefix ? p.prefix_splits : p.splits;
+  int unit = blockIdx.x, split = blockIdx.y;
+  if constexpr (MODE == kDecodeShared) {
+    unit -= is_prefix ? 0 : p.prefix_ctas;
+    split = unit % splits;
+    unit /= splits;
+  }
+  const int kvh = unit % p.num_kv_heads;
   int64_t b;          // the request whose table is read
   int64_t skip = 0;   // tokens before the range that the splits share
   int64_t len;        // length of that range (kDecodeSparse: of the selected chunks, end to end)
   int64_t ctx = 0;    // kDecodeSparse: the request's length
   RowTile rt{};
-  if constexpr (MODE == kDecodePrefix) {
-    rt = find_row_tile(p, static_cast<int>(blockIdx.x) / p.num_kv_heads, 16, lane);
+  if (is_prefix) {
+    rt = find_row_tile(p, unit / p.num_kv_heads, 16, lane);
     if (rt.prefix == 0) return;  // no such tile, or nothing shared
     b = rt.leader;
     len = rt.prefix;
   } else {
-    b = static_cast<int>(blockIdx.x) / p.num_kv_heads;
+    b = unit / p.num_kv_heads;
     len = clamped_len(p, b, threadIdx.x == 0 && split == 0);
-    if constexpr (MODE == kDecodeSuffix) {
+    if constexpr (MODE == kDecodeSuffix || MODE == kDecodeShared) {
       skip = shared_prefix_of(p, b, len, lane);
       len -= skip;
     }
@@ -431,7 +441,7 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     // equal shares of whole tiles: one wave of CTAs is what these launches ask for
     const int first = static_cast<int>(skip) / kMmaTile;
     const int total = len > 0 ? static_cast<int>(skip + len + kMmaTile - 1) / kMmaTile - first : 0;
-    const int each = total / p.splits, more = total - each * p.splits;
+    const int each = total / splits, more = total - each * splits;
     tile0 = first + split * each + (split < more ? split : more);
     n_tiles = each + (split < more ? 1 : 0);
     t_begin = tile0 * kMmaTile > skip ? tile0 * kMmaTile : skip;
@@ -441,7 +451,7 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
 
   const int r0 = lane >> 2, cq = (lane & 3) * 2;
   uint32_t qa[KS][4];
-  if constexpr (MODE == kDecodePrefix) {
+  if (is_prefix) {
     auto q_row = [&](int r) -> const T* {
       if (r >= (rt.end - rt.first) * p.group) return nullptr;
       return static_cast<const T*>(p.q) + (rt.first + r / p.group) * p.q_bs + (kvh * p.group + r % p.group) * p.q_hs;
@@ -595,12 +605,12 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     red[(w * 16 + r0 + 8) * SW + D + 1] = l_b;
   }
   __syncthreads();
-  const int rows = MODE == kDecodePrefix ? 16 : p.group;
+  const int rows = is_prefix ? 16 : p.group;
   for (int idx = threadIdx.x; idx < rows * D; idx += blockDim.x) {
     const int r = idx / D, d = idx % D;
     int64_t rb = b;
     int h = kvh * p.group + r;
-    if constexpr (MODE == kDecodePrefix) {
+    if (is_prefix) {
       const int row = static_cast<int>(rt.row0) + r;
       if (row >= (rt.end - rt.first) * p.group) continue;
       rb = rt.first + row / p.group;
@@ -629,7 +639,7 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
         ws[D + 1] = L;
       }
     } else {
-      const int64_t at = (rb * p.num_heads + h) * p.slots + p.slot0 + split;
+      const int64_t at = (rb * p.num_heads + h) * p.slots + (is_prefix ? 0 : p.slot0) + split;
       p.ws[at * D + d] = A;
       if (d == 0) p.ml[at] = make_float2(M, L);
     }
@@ -664,7 +674,7 @@ combine_partials_kernel(const MmaDecodeParams p) {
     if (part + k * WPR < p.slots) v[k] = ws[static_cast<int64_t>(part + k * WPR) * 32];
   const float2 first = lane < p.slots ? ml[lane] : make_float2(-INFINITY, 0.f);
   int s0 = 0;
-  if constexpr (MODE == kDecodeSuffix) {
+  if constexpr (MODE == kDecodeSuffix) {  // and after kDecodeShared
     if (shared_prefix_of(p, b, clamped_len(p, b, false), lane) == 0) s0 = p.slot0;
   }
   float M = lane >= s0 ? first.x : -INFINITY;
@@ -818,7 +828,8 @@ inline MmaDecodeParams mma_params(const nib_decode_attention_args& a, int splits
   return p;
 }
 
-// The kernel over `row_blocks` (request, kv head) pairs - kDecodePrefix: (row tile, kv head) - and p.splits splits.
+// The kernel over `row_blocks` (request, kv head) pairs and p.splits splits; kDecodeShared: over
+// `row_blocks` CTAs.
 // `after`: behind the kernel before it as a programmatic dependent.
 template <typename T, int D, int MODE>
 int launch_mma_mode(const nib_decode_attention_args& a, const MmaDecodeParams& p, int64_t row_blocks, cudaStream_t st,
@@ -841,7 +852,7 @@ int launch_mma_mode(const nib_decode_attention_args& a, const MmaDecodeParams& p
     }
     configured[dev] = static_cast<int>(smem);
   }
-  const dim3 grid(static_cast<unsigned>(row_blocks), static_cast<unsigned>(p.splits));
+  const dim3 grid(static_cast<unsigned>(row_blocks), MODE == kDecodeShared ? 1u : static_cast<unsigned>(p.splits));
   launch_k_pdl(after || pdl_enabled(), kernel, grid, kMmaWarps * 32, smem, st, kmap, vmap, p);
   return launch_status("decode_attention (tensor cores)");
 }

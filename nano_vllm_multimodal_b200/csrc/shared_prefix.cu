@@ -6,10 +6,11 @@
 // against the same K and V; over [P, len) each request has tokens of its own. Both halves
 // leave partials (max, sum, unnormalised output) that the combine kernel joins.
 //
-// Launches: the prefixes (row tiles x kv heads x splits), the suffixes (requests x kv heads x
-// splits), the combine. The suffix kernel reads nothing of the prefix kernel's: it starts as soon
-// as every CTA of that one has, on SMs that are free and as SMs become free, and waits for it only
-// before its own end, so that the combine follows both.
+// With few rows: one launch over the prefixes' row tiles (x kv heads x splits) and the suffixes
+// (requests x kv heads x splits), and the combine. With many: the prefixes by shared_prefix_tc.cu, the
+// suffixes, the combine. There the suffix kernel reads nothing of the prefix kernel's: it starts as
+// soon as every CTA of that one has, on SMs that are free and as SMs become free, and waits for it
+// only before its own end, so that the combine follows both.
 #include "decode_mma.cuh"
 
 namespace nib {
@@ -34,9 +35,18 @@ static SharedPrefixPlan shared_prefix_plan(const nib_shared_prefix_args& s) {
   const int64_t max_prefix = s.max_prefix_len > 0 && s.max_prefix_len < max_len ? s.max_prefix_len : max_len;
   // sum over the groups of ceil(rows / tile) <= (all rows + (tile - 1) groups) / tile
   const int64_t rows = a.batch * group;
-  pl.tc = a.variant == 2 || (a.variant == 0 && rows >= 32 * s.num_groups);
-  const int64_t tile = pl.tc ? prefix_tc_rows() : 16;
-  pl.row_tiles = (rows + (tile - 1) * s.num_groups) / tile;
+  auto row_tiles = [&](int64_t tile) { return (rows + (tile - 1) * s.num_groups) / tile; };
+  // The tcgen05 kernel reads a tile for up to 256 rows, the 16-row kernel for 16, but a CTA of the
+  // first has an SM to itself and takes microseconds to start and end: it runs with more than 32
+  // rows a group and at least 6,144 tokens x row tiles for each (group, kv head), and as many
+  // again for two. Measured, us a call, 16-row / tcgen05 kernel (16/2 heads of 128, 40 tokens
+  // behind the prefix): one group of 160 rows behind 1,024 tokens 15.0 / 16.1, 320 rows 20.5 / 17.3;
+  // 40 rows behind 4,096 tokens 19.0 / 15.7; five groups of 64 rows behind 1,024 tokens 18.3 / 23.9, of
+  // 128 rows 23.1 / 21.8; 16/8 heads: one group of 20 rows behind 16,384 tokens 26.4 / 29.1, of 40 rows
+  // 34.5 / 30.1.
+  pl.tc = a.variant == 2 || (a.variant == 0 && rows > 32 * s.num_groups &&
+                             row_tiles(16) * a.num_kv_heads * max_prefix >= 6144 * (s.num_groups * a.num_kv_heads + 2));
+  pl.row_tiles = row_tiles(pl.tc ? prefix_tc_rows() : 16);
   // as many splits as fit the SMs' three CTAs each at once, of at least `least` tokens: 64 requests
   // of up to 1,024 tokens behind 8,192 shared ones 57.4 us with 3 CTAs per SM wanted, 63.2 with 12;
   // 93 of up to 333 (fp16, D = 64) 24.7 us with 256 tokens at least, 28.4 with 64
@@ -80,15 +90,21 @@ static int launch_shared_prefix(const nib_shared_prefix_args& s, const SharedPre
   p.group_offsets = s.group_offsets;
   p.prefix_lens = s.prefix_lens;
   p.num_groups = static_cast<int>(s.num_groups);
-  if (s.num_groups > 0) {
-    const int rc = pl.tc ? launch_prefix_tc(a, p, pl.row_tiles, st)
-                         : launch_mma_mode<T, D, kDecodePrefix>(a, p, pl.row_tiles * a.num_kv_heads, st);
+  if (s.num_groups > 0 && pl.tc) {
+    const int rc = launch_prefix_tc(a, p, pl.row_tiles, st);
     if (rc != NIB_OK) return rc;
   }
+  p.prefix_splits = pl.prefix_splits;
   p.splits = pl.suffix_splits;
   p.slot0 = pl.prefix_splits;
-  p.early = s.num_groups > 0;
-  const int rc = launch_mma_mode<T, D, kDecodeSuffix>(a, p, a.batch * a.num_kv_heads, st, p.early);
+  int rc;
+  if (s.num_groups > 0 && !pl.tc) {
+    p.prefix_ctas = static_cast<int>(pl.row_tiles * a.num_kv_heads * pl.prefix_splits);
+    rc = launch_mma_mode<T, D, kDecodeShared>(a, p, p.prefix_ctas + a.batch * a.num_kv_heads * pl.suffix_splits, st);
+  } else {
+    p.early = s.num_groups > 0;
+    rc = launch_mma_mode<T, D, kDecodeSuffix>(a, p, a.batch * a.num_kv_heads, st, p.early);
+  }
   if (rc != NIB_OK) return rc;
   return launch_combine_partials<T, D, kDecodeSuffix>(a, p, st);
 }
@@ -124,7 +140,7 @@ extern "C" int nib_shared_prefix_decode_attention(const nib_shared_prefix_args* 
                   (s->num_groups == 0 || (s->group_offsets && s->prefix_lens)),
               "shared_prefix_decode_attention: null pointer");
   const int64_t group = a.num_heads / a.num_kv_heads;
-  NIB_REQUIRE((a.batch * group + s->num_groups) * a.num_kv_heads <= 0x7fffffffLL && a.batch * a.num_heads <= 0x7fffffffLL,
+  NIB_REQUIRE((a.batch * group + s->num_groups) * a.num_kv_heads <= (1LL << 24) && a.batch * a.num_heads <= (1LL << 24),
               "shared_prefix_decode_attention: batch too large");
   NIB_REQUIRE(a.max_blocks_per_seq * a.block_size < kMaxTokens,
               "shared_prefix_decode_attention: block table covers too many tokens (2^31 - 4096)");
