@@ -6,14 +6,17 @@
 // each stream has 128 of them and every tile; else both have the same rows and every other tile,
 // and join their sums at the end. For each of its tiles a stream runs
 //   S = Q K^T      128 x 128 x D, Q and K from shared memory, S in TMEM
-//   P = 2^(S - m)  four warps, a row per thread: no shuffles; P (bf16/f16) over S in TMEM
+//   P = 2^(S - m)  four warps, a row per thread: no shuffles; P over S in TMEM, in two halves of
+//                  the tile's tokens, so that the first half's product runs under the second's
+//                  exponentials. P is rounded to the cache's type (half a step of 2^-8 or 2^-11
+//                  relative, as the operand type of the product wants); its sum is of fp32 values
 //   O += P V       128 x D x 128, P from TMEM, V from shared memory, O in TMEM
-// m is the running maximum, raised only when a tile exceeds it by more than 2^8 (O and the sum
-// are then rescaled): P stays below 2^8 and the fp32 sums cancel the common factor.
+// m is the running maximum, raised only when a tile exceeds it by more than 8 in the exponent (O
+// and the sum are then rescaled): P stays at most 2^8 and the common factor cancels.
 //
 // Warps: 0 loads K and V tiles by TMA (5-D tensor maps over the paged cache, 128-byte swizzle,
-// no multicast) into a ring of five tiles, 1 issues the MMAs, 4-7 and 8-11 are the streams'
-// softmax. Shared memory (224 KB at D = 128) and the 512 TMEM columns (two S, two O) are all of
+// no multicast) into a ring of five tiles, 1 and 2 issue a stream's MMAs each, 4-7 and 8-11 are
+// the streams' softmax. Shared memory (224 KB at D = 128) and the 512 TMEM columns (two S, two O) are all of
 // an SM's, so one CTA runs there. K is the K-major B operand; V, whose rows run along d, the
 // MN-major one: no transposition is needed. All waits are bounded; on a timeout the CTA reports
 // NIB_DEV_TIMEOUT, lets its copies land, frees its TMEM and returns.
@@ -42,8 +45,8 @@ struct PtSmem {
 
 struct PtBars {
   uint64_t full[kPtSlots], empty[kPtSlots];
-  uint64_t s_full[2], p_full[2], o_done[2];
-  uint64_t turn[2][4];  // whose exponentials are next, per pair of warps on a scheduler
+  uint64_t s_full[2], p_half[2], p_full[2], o_done[2];
+  uint64_t turn[2][4];  // whose exponentials are next, per pair of warps that share a scheduler
   uint64_t landed;  // copies of a tile that is mended before it counts as full
   uint32_t tmem;
   int abort;
@@ -99,6 +102,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_half[i], 128);
       mbar_init(&bars.p_full[i], 128);
       mbar_init(&bars.o_done[i], 1);
       for (int k = 0; k < 4; ++k) mbar_init(&bars.turn[i][k], 1);
@@ -243,13 +247,23 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (int i = 0; ok && i < mine; ++i) {
       const int num = v_load(tile_of(s, i)), slot = num % kPtSlots;
       const int next = i + 1 < mine ? k_load(tile_of(s, i + 1)) : -1;
-      ok = wait_all(&bars.full[slot], static_cast<uint32_t>((num / kPtSlots) & 1)) && wait_all(&bars.p_full[s], static_cast<uint32_t>(i & 1));
+      // P comes in two halves of the tile's tokens: the first half's product runs while the second
+      // half's exponentials are computed
+      const uint32_t parity = static_cast<uint32_t>(i & 1);
+      ok = wait_all(&bars.full[slot], static_cast<uint32_t>((num / kPtSlots) & 1)) && wait_all(&bars.p_half[s], parity);
       if (!ok) break;
       tc_fence_after();
       const uint64_t v = v_desc + slot * (L::kSlot >> 4);
       if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < kPtTile / 16; ++kk) tc_mma_ts(to, ts + kk * 8, v + kk * (2048 >> 4), kIdO, i > 0 || kk > 0);
+        for (int kk = 0; kk < kPtTile / 32; ++kk) tc_mma_ts(to, ts + kk * 8, v + kk * (2048 >> 4), kIdO, i > 0 || kk > 0);
+      }
+      ok = wait_all(&bars.p_full[s], parity);
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int kk = kPtTile / 32; kk < kPtTile / 16; ++kk) tc_mma_ts(to, ts + kk * 8, v + kk * (2048 >> 4), kIdO, true);
         tc_commit(&bars.o_done[s]);
         tc_commit(&bars.empty[slot]);
       }
@@ -292,22 +306,26 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         for (int e = 0; e < 32; ++e)
           if (!((bits >> e) & 1u)) x[e] = 0xff800000u;
       };
-      uint32_t x[kPtTile];
-#pragma unroll
-      for (int c = 0; c < kPtTile / 32; ++c) tmem_ld32(ts + c * 32, x + c * 32);
-      tmem_wait_ld();
-      if (!whole) {
-#pragma unroll
-        for (int c = 0; c < kPtTile / 32; ++c) mask(x + c * 32, c);
-      }
+      // S is read twice, for the maximum and for P: a row of it does not stay in registers without
+      // spills (102 us instead of 100)
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < kPtTile; e += 8) {
+      for (int c = 0; c < kPtTile / 32; c += 2) {
+        uint32_t x[64];
+        tmem_ld32(ts + c * 32, x);
+        tmem_ld32(ts + c * 32 + 32, x + 32);
+        tmem_wait_ld();
+        if (!whole) {
+          mask(x, c);
+          mask(x + 32, c + 1);
+        }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], __uint_as_float(x[e + k]), __uint_as_float(x[e + 4 + k]));
+        for (int e = 0; e < 64; e += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top[k] = max3(top[k], __uint_as_float(x[e + k]), __uint_as_float(x[e + 4 + k]));
+        }
       }
-      float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-      mx *= qs;
+      const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * qs;
       if (i == 0) {
         m = mx;
       } else if (__any_sync(0xffffffffu, mx > m + kPtRaise)) {
@@ -330,8 +348,11 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
       }
       const float sub = m == -INFINITY ? 0.f : m;  // a row of nothing but masked tokens: all P are 0
-      // the streams take turns: stream 0's step i, stream 1's step i, stream 0's step i + 1, ...
-      if (s == 1 || i > 0) {
+      // Streams with rows of their own take turns with the exponentials (stream 0's step i, stream
+      // 1's step i, stream 0's step i + 1, ...): one computes while the other's products run. Left
+      // to themselves they fall into step (104 us instead of 100). Streams of the same rows, which
+      // wait for memory, are left alone.
+      if (both && (s == 1 || i > 0)) {
         ok = __all_sync(0xffffffffu, pt_wait(bars, &bars.turn[s][w & 3], static_cast<uint32_t>((s == 1 ? i : i - 1) & 1)));
         if (!ok) break;
       }
@@ -339,19 +360,31 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < kPtTile / 64; ++c) {
-        uint32_t pk[32];
+        uint32_t pk[32], x[64];
+        tmem_ld32(ts + c * 64, x);
+        tmem_ld32(ts + c * 64 + 32, x + 32);
+        tmem_wait_ld();
+        if (!whole) {
+          mask(x, 2 * c);
+          mask(x + 32, 2 * c + 1);
+        }
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const int k = c * 64 + 2 * e;
+          const int k = 2 * e;
           const float2 y = unpair2(fma2(pair2(x[k], x[k + 1]), qs2, sub2));
           const float a = ex2_fast(y.x), b = ex2_fast(y.y);
           part[e & 1] = add2(part[e & 1], pair2(a, b));
           pk[e] = pack2<T>(a, b);
         }
         tmem_st32(ts + c * 32, pk);
+        if (c == 0) {
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&bars.p_half[s]);
+        }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.turn[1 - s][w & 3]);
+      if (both && lane == 0) mbar_arrive(&bars.turn[1 - s][w & 3]);
       const float2 sum = unpair2(add2(part[0], part[1]));
       l += sum.x + sum.y;
       tmem_wait_st();
