@@ -15,7 +15,7 @@
 // and the sum are then rescaled): P stays at most 2^8 and the common factor cancels.
 //
 // Warps: 0 loads K and V tiles by TMA (5-D tensor maps over the paged cache, 128-byte swizzle,
-// no multicast) into a ring of five tiles, 1 and 2 issue a stream's MMAs each, 4-7 and 8-11 are
+// no multicast), 1 and 2 issue a stream's MMAs each, 4-7 and 8-11 are
 // the streams' softmax. Shared memory (224 KB at D = 128) and the 512 TMEM columns (two S, two O) are all of
 // an SM's, so one CTA runs there. K is the K-major B operand; V, whose rows run along d, the
 // MN-major one: no transposition is needed. All waits are bounded; on a timeout the CTA reports
@@ -28,7 +28,10 @@ namespace nib {
 constexpr int kPtThreads = 384;
 constexpr int kPtTile = 128;   // tokens per tile
 constexpr int kPtRows = 128;   // rows per stream
-constexpr int kPtSlots = 5;    // ring of K and V tiles
+// Shared memory holds seven tiles' worth: both streams' Q and a ring of five K and V tiles that both
+// read, or the one Q and a ring of three for each stream. (A ring's waits tell one use of a slot from
+// the next by parity alone, so whoever waits there has to take part in every use.)
+constexpr int kPtSlots = 6;
 constexpr float kPtRaise = 8.f;
 
 struct PrefixTcParams {
@@ -40,7 +43,8 @@ template <int D>
 struct PtSmem {
   static constexpr uint32_t kQ = kPtRows * D * 2;      // one stream's rows
   static constexpr uint32_t kSlot = kPtTile * D * 2;   // a K or V tile
-  static constexpr uint32_t kBytes = 2 * kQ + kPtSlots * kSlot + 1024;
+  static_assert(kQ == kSlot, "Q and tiles change places");
+  static constexpr uint32_t kBytes = 7 * kSlot + 1024;
 };
 
 struct PtBars {
@@ -111,68 +115,25 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     bars.abort = 0;
     fence_mbar_init();
   }
-  // stream s: its number of tiles and its i-th one; the ring's load number of tile t's K and V
-  // (in the order in which the MMAs want them; a number that has no tile is left out, and no
-  // later one comes round to its slot)
+  // stream s: its number of tiles and its i-th one; load 2 i brings that one's K, load 2 i + 1 its V
   auto steps = [&](int s) { return both ? n : (n + 1 - s) / 2; };
   auto tile_of = [&](int s, int i) { return both ? i : 2 * i + s; };
-  auto k_load = [&](int t) { return both ? 2 * t : t == 0 ? 0 : 2 * t - 1; };
-  auto v_load = [&](int t) { return both ? 2 * t + 1 : 2 * t + 2; };
+  const int slots = both ? 5 : 3;
+  auto slot_of = [&](int s, int num) { return both ? num % 5 : s * 3 + num % 3; };
+  auto phase_of = [&](int num) { return static_cast<uint32_t>((both ? num / 5 : num / 3) & 1); };
 
-  // ---- Q rows into shared memory (swizzled 128-byte rows, one 16 KB region per 64 channels)
-  {
-    constexpr int kVecs = D / 8, kTake = 2 * kPtRows * kVecs / kPtThreads + 1;  // vectors per thread
-    const uint32_t flip = p.qscale < 0.f ? 0x80008000u : 0u;  // the maximum is taken before the scale
-    const int have = (both ? 2 * kPtRows : kPtRows) * kVecs;
-    uint4 v[kTake];  // all of a thread's loads in flight
-#pragma unroll
-    for (int k = 0; k < kTake; ++k) {
-      const int e = threadIdx.x + k * kPtThreads, r = e / kVecs, row = row0 + r;
-      v[k] = zero_vec();
-      if (e < have && r < rows) {
-        const int request = row / p.group;
-        v[k] = ld_vec(static_cast<const T*>(p.q) + (rt.first + request) * p.q_bs +
-                      (kvh * p.group + row - request * p.group) * p.q_hs + e % kVecs * 8);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kTake; ++k) {
-      const int e = threadIdx.x + k * kPtThreads, r = e / kVecs, c = e % kVecs, in = r % kPtRows;
-      const uint32_t at = (r / kPtRows) * L::kQ + (c / 8) * (kPtRows * 128) + in * 128 + (((c % 8) ^ (in & 7)) << 4);
-      if (e < have) *reinterpret_cast<uint4*>(dsm + at) = make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip);
-    }
-    fence_proxy_async();
-  }
-  if (w == 1) tmem_alloc(&bars.tmem, 512);
-  tc_fence_before();
+  const uint32_t ring = base + (both ? 2 : 1) * L::kQ;
+  unsigned char* const ring_ptr = dsm + (both ? 2 : 1) * L::kQ;
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars.tmem;
-  const uint32_t ring = base + 2 * L::kQ;
 
   if (w == 0) {
     // ---------------------------------------------------------------- loads
     const int boxes = kPtTile / pp.box;
     const uint32_t box_bytes = static_cast<uint32_t>(pp.box) * D * 2;
-    const int loads = n > 0 ? (both ? 2 * n : 2 * n + 1) : 0;
     uint32_t landed_phase = 0;
-    for (int num = 0; num < loads; ++num) {
-      // which tile this load brings
-      bool is_v;
-      int t;
-      if (both) {
-        is_v = num & 1;
-        t = num >> 1;
-      } else if (num < 2) {
-        is_v = false;
-        t = num;
-      } else {
-        is_v = (num & 1) == 0;
-        t = is_v ? (num - 2) >> 1 : (num + 1) >> 1;
-      }
-      if (t >= n) continue;
-      const int slot = num % kPtSlots;
-      const int tok = (tile0 + t) * kPtTile, at = tok + lane * pp.box;
+    auto load = [&](int s, int num) -> bool {
+      const bool is_v = num & 1;
+      const int slot = slot_of(s, num), tok = (tile0 + tile_of(s, num >> 1)) * kPtTile, at = tok + lane * pp.box;
       int page = -1;
       if (lane < boxes && at < prefix) {
         page = __ldg(table + at / p.block_size);
@@ -184,8 +145,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
       const bool whole = __popc(have) == boxes && tok + kPtTile <= prefix;
       bool ok = true;
-      if (num >= kPtSlots) ok = pt_wait(bars, &bars.empty[slot], static_cast<uint32_t>((num / kPtSlots - 1) & 1));
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (num >= slots) ok = pt_wait(bars, &bars.empty[slot], phase_of(num - slots));
+      if (!__all_sync(0xffffffffu, ok)) return false;
       const bool mend = is_v && !whole;  // rows behind the prefix or without a page become zeros: 0 x NaN is NaN
       uint64_t* bar = mend ? &bars.landed : &bars.full[slot];
       if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * box_bytes);
@@ -200,18 +161,63 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       if (mend) {
         ok = pt_wait(bars, &bars.landed, landed_phase);
         landed_phase ^= 1;
-        if (!__all_sync(0xffffffffu, ok)) break;
+        if (!__all_sync(0xffffffffu, ok)) return false;
         for (int e = lane; e < kPtTile * (D / 8); e += 32) {
           const int row = e % kPtTile, c = e / kPtTile;
           if (tok + row >= prefix || !((have >> (row / pp.box)) & 1u))
-            *reinterpret_cast<uint4*>(dsm + 2 * L::kQ + slot * L::kSlot + (c / 8) * (kPtTile * 128) + row * 128 + (c % 8) * 16) = zero_vec();
+            *reinterpret_cast<uint4*>(ring_ptr + slot * L::kSlot + (c / 8) * (kPtTile * 128) + row * 128 + (c % 8) * 16) = zero_vec();
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.full[slot]);
       }
+      return true;
+    };
+    if (both) {
+      for (int num = 0; num < 2 * n; ++num)
+        if (!load(0, num)) break;
+    } else {  // K of a stream's first tile, then V of each tile and K of the next, the streams by turns
+      bool ok = true;
+      for (int i = 0; ok && i <= steps(0); ++i)
+        for (int s = 0; ok && s < 2; ++s) {
+          if (i > 0 && i - 1 < steps(s)) ok = load(s, 2 * i - 1);
+          if (ok && i < steps(s)) ok = load(s, 2 * i);
+        }
     }
-  } else if (w <= 2) {
+  } else {
+    // ---- Q rows into shared memory (swizzled 128-byte rows, one 16 KB region per 64 channels),
+    // while warp 0's first tiles are under way
+    if (w == 1) tmem_alloc(&bars.tmem, 512);
+    {
+      constexpr int kTakers = kPtThreads - 32, kVecs = D / 8;
+      constexpr int kTake = (2 * kPtRows * kVecs + kTakers - 1) / kTakers;  // vectors per thread
+      const uint32_t flip = p.qscale < 0.f ? 0x80008000u : 0u;  // the maximum is taken before the scale
+      const int have = (both ? 2 * kPtRows : kPtRows) * kVecs;
+      uint4 v[kTake];  // all of a thread's loads in flight
+#pragma unroll
+      for (int k = 0; k < kTake; ++k) {
+        const int e = threadIdx.x - 32 + k * kTakers, r = e / kVecs, row = row0 + r;
+        v[k] = zero_vec();
+        if (e < have && r < rows) {
+          const int request = row / p.group;
+          v[k] = ld_vec(static_cast<const T*>(p.q) + (rt.first + request) * p.q_bs +
+                        (kvh * p.group + row - request * p.group) * p.q_hs + e % kVecs * 8);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kTake; ++k) {
+        const int e = threadIdx.x - 32 + k * kTakers, r = e / kVecs, c = e % kVecs, in = r % kPtRows;
+        const uint32_t at = (r / kPtRows) * L::kQ + (c / 8) * (kPtRows * 128) + in * 128 + (((c % 8) ^ (in & 7)) << 4);
+        if (e < have) *reinterpret_cast<uint4*>(dsm + at) = make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip);
+      }
+      fence_proxy_async();
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 2, %0;" ::"n"(kPtThreads - 32) : "memory");
+    tc_fence_after();
+  }
+  const uint32_t tmem = bars.tmem;
+  if (w == 1 || w == 2) {
     // ---------------------------------------------------------------- MMAs, a warp per stream
     // The whole warp runs the loop and waits; one lane issues. Operand addresses change in the
     // descriptors' low words only.
@@ -223,9 +229,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     const uint64_t k_desc = smem_desc(ring, 16, 1024), v_desc = smem_desc(ring, kPtTile * 128, 1024);
     const bool leader = elect_one();
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, pt_wait(bars, bar, parity)) != 0; };
-    auto scores = [&](int num) {  // S = Q K^T, K by the ring's load `num`
+    auto scores = [&](int num) {  // S = Q K^T, K by load `num`
       tc_fence_after();
-      const int slot = num % kPtSlots;
+      const int slot = slot_of(s, num);
       const uint64_t k = k_desc + slot * (L::kSlot >> 4);
       if (leader) {
 #pragma unroll
@@ -240,17 +246,15 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     };
     bool ok = true;
     if (mine > 0) {
-      const int num = k_load(tile_of(s, 0));
-      ok = wait_all(&bars.full[num % kPtSlots], static_cast<uint32_t>((num / kPtSlots) & 1));
-      if (ok) scores(num);
+      ok = wait_all(&bars.full[slot_of(s, 0)], 0);
+      if (ok) scores(0);
     }
     for (int i = 0; ok && i < mine; ++i) {
-      const int num = v_load(tile_of(s, i)), slot = num % kPtSlots;
-      const int next = i + 1 < mine ? k_load(tile_of(s, i + 1)) : -1;
+      const int num = 2 * i + 1, slot = slot_of(s, num), next = i + 1 < mine ? num + 1 : -1;
       // P comes in two halves of the tile's tokens: the first half's product runs while the second
       // half's exponentials are computed
       const uint32_t parity = static_cast<uint32_t>(i & 1);
-      ok = wait_all(&bars.full[slot], static_cast<uint32_t>((num / kPtSlots) & 1)) && wait_all(&bars.p_half[s], parity);
+      ok = wait_all(&bars.full[slot], phase_of(num)) && wait_all(&bars.p_half[s], parity);
       if (!ok) break;
       tc_fence_after();
       const uint64_t v = v_desc + slot * (L::kSlot >> 4);
@@ -269,7 +273,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       if (next >= 0) {
         // the next scores overwrite P: only after the product that reads it
-        ok = wait_all(&bars.full[next % kPtSlots], static_cast<uint32_t>((next / kPtSlots) & 1)) &&
+        ok = wait_all(&bars.full[slot_of(s, next)], phase_of(next)) &&
              wait_all(&bars.o_done[s], static_cast<uint32_t>(i & 1));
         if (ok) scores(next);
       }
@@ -395,7 +399,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     tc_fence_after();
     // ---- partials: rows of their own go straight to the workspace; streams of the same rows
     // meet in shared memory (the ring is free: every tile in it has been used)
-    float* meet = reinterpret_cast<float*>(dsm + 2 * L::kQ);
+    float* meet = reinterpret_cast<float*>(ring_ptr);
     const int r = (w & 3) * 32 + lane;
     if (!both) {
       asm volatile("bar.sync 1, 256;" ::: "memory");  // both streams' last products have ended

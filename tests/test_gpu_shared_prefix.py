@@ -104,6 +104,26 @@ def test_long_prefix_and_many_splits():
         _check(c, _call(c, max_prefix_len=20000, max_context_len=20700, variant=variant))
 
 
+@pytest.mark.parametrize("nq,nkv,requests", [(16, 8, 64), (16, 2, 40)])
+def test_repeated_calls_give_the_same_bits(nq, nkv, requests):
+    """Tiles land in any order when the cache comes from memory: one CTA's long run of tiles, for 128
+    rows (two streams of the same rows) and for more, repeated behind other traffic. Hints below the
+    prefix's length leave each CTA more tiles."""
+    c = _case(requests, nq, nkv, 128, 64, [(12000, [i % 7 for i in range(requests)])], [], poison=False)
+    cu = {k: (v.cuda() if torch.is_tensor(v) else v) for k, v in c.items()}
+    other = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for hint in (12000, 3000, 500):
+        first = None
+        for i in range(15):
+            if i % 3:
+                other.fill_(i)
+            out = ops.shared_prefix_decode_attention(*(cu[k] for k in ("q", "kc", "vc", "lens", "tables", "offsets", "prefix")),
+                                                     c["scale"], max_prefix_len=hint, variant=ops.PREFIX_ROWS256)
+            first = out if first is None else first
+            assert torch.equal(out, first), (hint, i)
+        _check(c, first, f"hint {hint}")
+
+
 @pytest.mark.parametrize("requests", [130, 300])
 def test_many_requests(requests):
     c = _case(requests, 16, 2, 128, 64, [(1500, [i % 50 for i in range(requests)])], [])
