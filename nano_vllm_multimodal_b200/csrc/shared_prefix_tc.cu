@@ -28,9 +28,10 @@ namespace nib {
 constexpr int kPtThreads = 384;
 constexpr int kPtTile = 128;   // tokens per tile
 constexpr int kPtRows = 128;   // rows per stream
-// Shared memory holds seven tiles' worth: both streams' Q and a ring of five K and V tiles that both
-// read, or the one Q and a ring of three for each stream. (A ring's waits tell one use of a slot from
-// the next by parity alone, so whoever waits there has to take part in every use.)
+// Shared memory holds seven tiles' worth: Q of each stream that has rows of its own, and a ring of K
+// and V tiles in what is left (five or six). A ring's waits tell one use of a slot from the next by
+// parity alone, so each stream waits for every load in order and gives every slot back, those of the
+// other stream's tiles unused.
 constexpr int kPtSlots = 6;
 constexpr float kPtRaise = 8.f;
 
@@ -102,7 +103,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPtSlots; ++i) {
       mbar_init(&bars.full[i], 1);
-      mbar_init(&bars.empty[i], both ? 2 : 1);  // the streams that use a tile
+      mbar_init(&bars.empty[i], 2);  // both streams
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
@@ -115,12 +116,14 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     bars.abort = 0;
     fence_mbar_init();
   }
-  // stream s: its number of tiles and its i-th one; load 2 i brings that one's K, load 2 i + 1 its V
+  // stream s: its number of tiles and its i-th one; the ring's load number of tile t's K and V, in
+  // the order in which the MMAs want them (a number without a tile is left out)
   auto steps = [&](int s) { return both ? n : (n + 1 - s) / 2; };
   auto tile_of = [&](int s, int i) { return both ? i : 2 * i + s; };
-  const int slots = both ? 5 : 3;
-  auto slot_of = [&](int s, int num) { return both ? num % 5 : s * 3 + num % 3; };
-  auto phase_of = [&](int num) { return static_cast<uint32_t>((both ? num / 5 : num / 3) & 1); };
+  auto k_load = [&](int t) { return both ? 2 * t : t == 0 ? 0 : 2 * t - 1; };
+  auto v_load = [&](int t) { return both ? 2 * t + 1 : 2 * t + 2; };
+  const int loads = n > 0 ? (both ? 2 * n : 2 * n + 1) : 0, left_out = both ? -1 : 2 * n - 1;
+  const int slots = both ? 5 : 6;
 
   const uint32_t ring = base + (both ? 2 : 1) * L::kQ;
   unsigned char* const ring_ptr = dsm + (both ? 2 : 1) * L::kQ;
@@ -130,10 +133,13 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     // ---------------------------------------------------------------- loads
     const int boxes = kPtTile / pp.box;
     const uint32_t box_bytes = static_cast<uint32_t>(pp.box) * D * 2;
-    uint32_t landed_phase = 0;
-    auto load = [&](int s, int num) -> bool {
-      const bool is_v = num & 1;
-      const int slot = slot_of(s, num), tok = (tile0 + tile_of(s, num >> 1)) * kPtTile, at = tok + lane * pp.box;
+    uint32_t landed_phase = 0, phase = 1;  // the parity of a slot's release, one use behind
+    int slot = 0;
+    for (int num = 0; num < loads; ++num, phase ^= slot + 1 == slots, slot = slot + 1 == slots ? 0 : slot + 1) {
+      if (num == left_out) continue;
+      const bool is_v = both || num < 2 ? (both && (num & 1)) : (num & 1) == 0;
+      const int t = both ? num >> 1 : num < 2 ? num : is_v ? (num - 2) >> 1 : (num + 1) >> 1;
+      const int tok = (tile0 + t) * kPtTile, at = tok + lane * pp.box;
       int page = -1;
       if (lane < boxes && at < prefix) {
         page = __ldg(table + at / p.block_size);
@@ -145,8 +151,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
       const bool whole = __popc(have) == boxes && tok + kPtTile <= prefix;
       bool ok = true;
-      if (num >= slots) ok = pt_wait(bars, &bars.empty[slot], phase_of(num - slots));
-      if (!__all_sync(0xffffffffu, ok)) return false;
+      if (num >= slots) ok = pt_wait(bars, &bars.empty[slot], phase);
+      if (!__all_sync(0xffffffffu, ok)) break;
       const bool mend = is_v && !whole;  // rows behind the prefix or without a page become zeros: 0 x NaN is NaN
       uint64_t* bar = mend ? &bars.landed : &bars.full[slot];
       if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * box_bytes);
@@ -161,7 +167,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       if (mend) {
         ok = pt_wait(bars, &bars.landed, landed_phase);
         landed_phase ^= 1;
-        if (!__all_sync(0xffffffffu, ok)) return false;
+        if (!__all_sync(0xffffffffu, ok)) break;
         for (int e = lane; e < kPtTile * (D / 8); e += 32) {
           const int row = e % kPtTile, c = e / kPtTile;
           if (tok + row >= prefix || !((have >> (row / pp.box)) & 1u))
@@ -171,18 +177,6 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.full[slot]);
       }
-      return true;
-    };
-    if (both) {
-      for (int num = 0; num < 2 * n; ++num)
-        if (!load(0, num)) break;
-    } else {  // K of a stream's first tile, then V of each tile and K of the next, the streams by turns
-      bool ok = true;
-      for (int i = 0; ok && i <= steps(0); ++i)
-        for (int s = 0; ok && s < 2; ++s) {
-          if (i > 0 && i - 1 < steps(s)) ok = load(s, 2 * i - 1);
-          if (ok && i < steps(s)) ok = load(s, 2 * i);
-        }
     }
   } else {
     // ---- Q rows into shared memory (swizzled 128-byte rows, one 16 KB region per 64 channels),
@@ -229,35 +223,46 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     const uint64_t k_desc = smem_desc(ring, 16, 1024), v_desc = smem_desc(ring, kPtTile * 128, 1024);
     const bool leader = elect_one();
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, pt_wait(bars, bar, parity)) != 0; };
-    auto scores = [&](int num) {  // S = Q K^T, K by load `num`
+    // waits for the loads up to `num` in order; the slot of that one
+    int seen = 0, at = -1;
+    uint32_t phase = 1;
+    auto reach = [&](int num) -> bool {
+      for (; seen <= num; ++seen) {
+        at = at + 1 == slots ? 0 : at + 1;
+        phase ^= at == 0;
+        if (seen == left_out) continue;
+        if (!wait_all(&bars.full[at], phase)) return false;
+        if (seen < num && leader) mbar_arrive(&bars.empty[at]);  // the other stream's
+      }
       tc_fence_after();
-      const int slot = slot_of(s, num);
-      const uint64_t k = k_desc + slot * (L::kSlot >> 4);
+      return true;
+    };
+    auto scores = [&]() {  // S = Q K^T, K by the load reached
+      const uint64_t k = k_desc + at * (L::kSlot >> 4);
       if (leader) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           constexpr uint32_t kHalf = kPtRows * 128;
-          const uint32_t at = ((kk / 4) * kHalf + (kk % 4) * 32) >> 4;
-          tc_mma_ss(ts, q_desc + at, k + at, kIdS, kk > 0);
+          const uint32_t in = ((kk / 4) * kHalf + (kk % 4) * 32) >> 4;
+          tc_mma_ss(ts, q_desc + in, k + in, kIdS, kk > 0);
         }
         tc_commit(&bars.s_full[s]);
-        tc_commit(&bars.empty[slot]);
+        tc_commit(&bars.empty[at]);
       }
     };
     bool ok = true;
     if (mine > 0) {
-      ok = wait_all(&bars.full[slot_of(s, 0)], 0);
-      if (ok) scores(0);
+      ok = reach(k_load(tile_of(s, 0)));
+      if (ok) scores();
     }
     for (int i = 0; ok && i < mine; ++i) {
-      const int num = 2 * i + 1, slot = slot_of(s, num), next = i + 1 < mine ? num + 1 : -1;
       // P comes in two halves of the tile's tokens: the first half's product runs while the second
       // half's exponentials are computed
       const uint32_t parity = static_cast<uint32_t>(i & 1);
-      ok = wait_all(&bars.full[slot], phase_of(num)) && wait_all(&bars.p_half[s], parity);
+      ok = reach(v_load(tile_of(s, i))) && wait_all(&bars.p_half[s], parity);
       if (!ok) break;
       tc_fence_after();
-      const uint64_t v = v_desc + slot * (L::kSlot >> 4);
+      const uint64_t v = v_desc + at * (L::kSlot >> 4);
       if (leader) {
 #pragma unroll
         for (int kk = 0; kk < kPtTile / 32; ++kk) tc_mma_ts(to, ts + kk * 8, v + kk * (2048 >> 4), kIdO, i > 0 || kk > 0);
@@ -269,13 +274,12 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 #pragma unroll
         for (int kk = kPtTile / 32; kk < kPtTile / 16; ++kk) tc_mma_ts(to, ts + kk * 8, v + kk * (2048 >> 4), kIdO, true);
         tc_commit(&bars.o_done[s]);
-        tc_commit(&bars.empty[slot]);
+        tc_commit(&bars.empty[at]);
       }
-      if (next >= 0) {
+      if (i + 1 < mine) {
         // the next scores overwrite P: only after the product that reads it
-        ok = wait_all(&bars.full[slot_of(s, next)], phase_of(next)) &&
-             wait_all(&bars.o_done[s], static_cast<uint32_t>(i & 1));
-        if (ok) scores(next);
+        ok = reach(k_load(tile_of(s, i + 1))) && wait_all(&bars.o_done[s], parity);
+        if (ok) scores();
       }
     }
   } else if (w >= 4) {
