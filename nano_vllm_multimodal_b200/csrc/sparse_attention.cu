@@ -41,9 +41,12 @@ constexpr int kBoundsThreads = 256;
 constexpr int kBoundsUnroll = 8;
 
 // One CTA per (window of a request, request): the window's chunk over all kv heads. A thread
-// owns one 16-byte vector of the token row (8 channels of a head) and every slices-th token.
+// owns one 16-byte vector of the token row (8 channels of a head) and every slices-th token, eight
+// loads in flight. Bound by HBM for long prefills; three CTAs per SM (16 x 16,384 tokens of 8 x 128
+// 87.5 us, 256 single steps 6.3 us) against four, whose registers spill (85.0 and 7.4), and four with
+// four loads in flight (113.6 and 10.0).
 template <typename T, int D>
-__global__ void __launch_bounds__(kBoundsThreads, 4)
+__global__ void __launch_bounds__(kBoundsThreads, 3)
 key_bounds_kernel(const BoundsParams p) {
   pdl_enter();
   using V2 = typename Vec2<T>::type;
