@@ -438,7 +438,7 @@ static DecodePlan decode_plan(const nib_decode_attention_args& a) {
   // with 256 requests 0.658 with one split, 0.641 with two.
   const int64_t ctas = a.batch * a.num_kv_heads;
   const int64_t want = (pl.mma ? 12LL : 4LL) * sm_count();
-  int64_t s = ctas >= want ? 1 : (want + ctas - 1) / ctas;
+  int64_t s = ctas < 1 || ctas >= want ? 1 : (want + ctas - 1) / ctas;  // an empty batch asks for nothing
   if (pl.mma && s < 2) s = 2;
   const int64_t max_len = a.max_context_len > 0 ? a.max_context_len : a.max_blocks_per_seq * a.block_size;
   const int64_t by_len = (max_len + (pl.mma ? 63 : 255)) / (pl.mma ? 64 : 256);

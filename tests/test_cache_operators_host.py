@@ -90,6 +90,11 @@ def test_attention_arguments(lib):
     assert lib.nib_sparse_decode_workspace_bytes(ctypes.byref(s)) >= keys
 
 
+def test_decode_workspace_of_an_empty_batch(lib):
+    lib.nib_decode_attention_workspace_bytes.restype = i64
+    assert lib.nib_decode_attention_workspace_bytes(ctypes.byref(_decode(batch=0))) == 0
+
+
 def test_page_arguments(lib):
     bad = [
         (lib.nib_paged_copy_blocks, (SOME, i64(2), i64(1 << 20), i64(4), i64(64), None, None, i64(1), None, None), "null pointer"),
