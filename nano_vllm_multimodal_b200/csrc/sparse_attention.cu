@@ -547,9 +547,10 @@ chunk_select_kernel(const SelectParams p) {
   if (ranked) {
     constexpr int LPC = ScoreLanes<D>::kLanes, CPS = ScoreLanes<D>::kChunks;
     const int32_t* table = p.d.tables + b * p.d.table_stride;
-    double wt[8];
-    score_weights<T, D>(p, b, kvh, lane, wt);
     const int candidates = few ? band : n;
+    // only in the warps that score one: a row of 8 heads takes eight warps 10 us on the 64-bit pipe
+    double wt[8];
+    if (w * CPS < candidates) score_weights<T, D>(p, b, kvh, lane, wt);
     for (int j0 = w * CPS; j0 < candidates; j0 += kSelectWarps * CPS) {
       const int j = j0 + lane / LPC;
       const int i = j >= candidates ? -1 : few ? s.at[j] : competes(j) ? j : -1;
