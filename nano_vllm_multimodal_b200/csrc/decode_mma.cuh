@@ -283,8 +283,9 @@ __device__ __forceinline__ void load_q_frags(uint32_t (&qa)[D / 16][4], const T*
 
 // One 16-token tile of a stage (K at kt, V at kt + tile bytes) into the online
 // softmax state of rows r0 (a) and r0 + 8 (b): S = Q K^T, scores of tokens
-// outside [lo, hi) (tile-relative) masked, then O += P V.
-template <typename T, int D>
+// outside [lo, hi) (tile-relative) masked, then O += P V. KEEP_NAN: a row whose scores are all NaN so
+// far keeps a NaN in its sum (and, below, in the result); without, it counts as empty.
+template <typename T, int D, bool KEEP_NAN>
 __device__ __forceinline__ void mma_tile(const uint32_t (&qa)[D / 16][4], uint32_t kt, int lo, int hi, float qscale,
                                          float (&o)[D / 8][4], float& m_a, float& m_b, float& l_a, float& l_b,
                                          int lane) {
@@ -335,8 +336,9 @@ __device__ __forceinline__ void mma_tile(const uint32_t (&qa)[D / 16][4], uint32
   for (int nt = 0; nt < 2; ++nt) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      pa[nt][c] = na == -INFINITY ? 0.f : ex2_fast(s[nt][c] - na);
-      pb[nt][c] = nb == -INFINITY ? 0.f : ex2_fast(s[nt][c + 2] - nb);
+      pa[nt][c] = na == -INFINITY ? (KEEP_NAN && s[nt][c] != s[nt][c] ? s[nt][c] : 0.f) : ex2_fast(s[nt][c] - na);
+      pb[nt][c] = nb == -INFINITY ? (KEEP_NAN && s[nt][c + 2] != s[nt][c + 2] ? s[nt][c + 2] : 0.f)
+                                  : ex2_fast(s[nt][c + 2] - nb);
     }
   }
   l_a = l_a * ra + (pa[0][0] + pa[0][1]) + (pa[1][0] + pa[1][1]);
@@ -574,7 +576,7 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     const int lo = from > t0 ? static_cast<int>(from - t0) : 0;
     const int hi = to - t0 < kMmaTile ? static_cast<int>(to - t0) : kMmaTile;
     if (lo > 0 || hi < kMmaTile) zero_rows<D>(dsm + (kt - base_all), lo, hi, lane);
-    mma_tile<T, D>(qa, kt, lo, hi, p.qscale, o, m_a, m_b, l_a, l_b, lane);
+    mma_tile<T, D, MODE != kDecodeFull>(qa, kt, lo, hi, p.qscale, o, m_a, m_b, l_a, l_b, lane);
     __syncwarp();  // every lane has read the stage before it is refilled
   }
 
@@ -628,9 +630,13 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
         L += rr[D + 1] * f;
         A += rr[d] * f;
       }
+    } else if (MODE != kDecodeFull) {
+#pragma unroll
+      for (int ww = 0; ww < kMmaWarps; ++ww) L += red[(ww * 16 + r) * SW + D + 1];  // 0, or the NaN of NaN scores
     }
     if (p.ws == nullptr) {
-      static_cast<T*>(p.out)[rb * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
+      const float none = MODE != kDecodeFull && L != L ? L : 0.f;
+      static_cast<T*>(p.out)[rb * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : none);
     } else if constexpr (MODE == kDecodeFull) {
       float* ws = p.ws + ((rb * p.num_heads + h) * p.splits + split) * SW;
       ws[d] = A;
@@ -682,10 +688,14 @@ combine_partials_kernel(const MmaDecodeParams p) {
     if (s >= s0) M = fmaxf(M, ml[s].x);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  // a NaN sum (of NaN scores) makes the row NaN
+  bool odd = lane >= s0 && first.y != first.y;
+  for (int s = 32 + lane; s < p.slots; s += 32) odd |= s >= s0 && ml[s].y != ml[s].y;
+  odd = __any_sync(0xffffffffu, odd);
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (M != -INFINITY) {
+  if (M != -INFINITY && !odd) {
     // a split without tokens has no output and the weight 0
     auto weight = [&](float2 x, int s) { return s >= s0 && x.x != -INFINITY ? ex2_fast(x.x - M) : 0.f; };
     const float f = weight(first, lane);
@@ -714,11 +724,12 @@ combine_partials_kernel(const MmaDecodeParams p) {
     }
   }
   T* out = static_cast<T*>(p.out) + b * p.o_bs + h * p.o_hs;
+  const float none = odd ? __int_as_float(0x7fffffff) : 0.f;
   if constexpr (WPR == 1) {
 #pragma unroll
     for (int e = 0; e < E; e += 2)
       *reinterpret_cast<typename Vec2<T>::type*>(out + lane * E + e) =
-          Vec2<T>::make(L > 0.f ? acc[e] / L : 0.f, L > 0.f ? acc[e + 1] / L : 0.f);
+          Vec2<T>::make(L > 0.f ? acc[e] / L : none, L > 0.f ? acc[e + 1] / L : none);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) red[w][lane * E + e] = acc[e];
@@ -728,7 +739,7 @@ combine_partials_kernel(const MmaDecodeParams p) {
       float A = 0.f;
 #pragma unroll
       for (int ww = 0; ww < kCombineWarps; ++ww) A += red[ww][d];
-      out[d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
+      out[d] = Elem<T>::from_f(L > 0.f ? A / L : none);
     }
   }
 }

@@ -261,6 +261,41 @@ def test_captured_replayed_and_on_two_streams():
         _check(c, o)
 
 
+@pytest.mark.parametrize("variant", [ops.PREFIX_ROWS16, ops.PREFIX_ROWS256])
+def test_nan_reaches_the_rows_that_meet_it_and_no_others(variant):
+    """A NaN query, a NaN key among the shared tokens (one kv head) and one behind them: NaN in
+    exactly the rows whose attention meets one."""
+    c = _case(16, 16, 8, 128, 16, [(300, [5, 40, 3])], [20], poison=True)
+    c["q"][1, 7] = float("nan")
+    c["kc"][c["tables"][0, 3], 2, 5, 9] = float("nan")   # shared: heads 10 and 11 of requests 0, 1, 2
+    c["kc"][c["tables"][3, 0], 1, 0, 0] = float("nan")   # heads 0 and 1 of request 3
+    expect = torch.zeros(4, 16, dtype=torch.bool)
+    expect[1, 7] = expect[3, :2] = True
+    expect[:3, 10:12] = True
+    out = _call(c, variant=variant).cpu()
+    assert torch.equal(torch.isnan(out).all(-1), expect) and torch.equal(torch.isnan(out).any(-1), expect)
+
+
+@pytest.mark.parametrize("variant", [ops.PREFIX_ROWS16, ops.PREFIX_ROWS256])
+def test_large_calls_on_two_streams(variant):
+    cases = [_case(70 + s, 16, 2, 128, 64, [(3000, [i % 9 for i in range(n)])], [], poison=False) for s, n in enumerate((60, 35))]
+    gpu = [{k: (v.cuda() if torch.is_tensor(v) else v) for k, v in c.items()} for c in cases]
+    call = lambda d: ops.shared_prefix_decode_attention(  # noqa: E731
+        *(d[k] for k in ("q", "kc", "vc", "lens", "tables", "offsets", "prefix", "scale")), variant=variant)
+    alone = [call(d) for d in gpu]
+    streams = [torch.cuda.Stream() for _ in gpu]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        outs = []
+        for s, d in zip(streams, gpu):
+            with torch.cuda.stream(s):
+                outs.append(call(d))
+    torch.cuda.synchronize()
+    for c, a, o in zip(cases, alone, outs):
+        assert torch.equal(a, o)
+        _check(c, o)
+
+
 def test_reports(monkeypatch):
     monkeypatch.setenv("NANOINFER_B200_VALIDATE", "1")
     c = _case(30, 16, 8, 128, 16, [(40, [3, 4])], [5], poison=False)

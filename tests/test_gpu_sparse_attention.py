@@ -260,6 +260,18 @@ def test_captured_replayed_and_on_two_streams():
         _check(c, 9, *o)
 
 
+@pytest.mark.parametrize("top", [3, 40])
+def test_nan_reaches_the_rows_that_meet_it_and_no_others(top):
+    """A NaN query (its kv head's selection is the lowest indices) and a NaN key in a selected chunk."""
+    c = _case(66, 16, 8, 128, 64, 16, [500, 333], poison=True)
+    c["q"][0, 5] = float("nan")
+    c["kc"][c["tables"][1, 0], 3, 7, 1] = float("nan")   # the first chunk is always selected: heads 14, 15
+    out = _call(c, top)[0].cpu()
+    expect = torch.zeros(2, 16, dtype=torch.bool)
+    expect[0, 5] = expect[1, 14] = expect[1, 15] = True
+    assert torch.equal(torch.isnan(out).all(-1), expect) and torch.equal(torch.isnan(out).any(-1), expect)
+
+
 def test_reports(monkeypatch):
     monkeypatch.setenv("NANOINFER_B200_VALIDATE", "1")
     c = _case(60, 16, 8, 128, 16, 16, [200, 100], poison=False)
