@@ -272,6 +272,33 @@ def test_nan_reaches_the_rows_that_meet_it_and_no_others(top):
     assert torch.equal(torch.isnan(out).all(-1), expect) and torch.equal(torch.isnan(out).any(-1), expect)
 
 
+def test_pages_past_32_bit_offsets():
+    """The same pages at the end of caches of 2.4e9 elements give the same bits, for the bounds, the
+    sparse and the shared-prefix attention."""
+    c = _case(67, 16, 8, 128, 256, 32, [1500, 700], poison=False)
+    small = c["kc"].shape[0]
+    pages = 9200  # x 256 x 8 x 128 elements
+    big = {k: torch.zeros(pages, 256, 8, 128, dtype=torch.bfloat16, device="cuda") for k in ("kc", "vc")}
+    for k in big:
+        big[k][pages - small:] = c[k].cuda()
+    moved = torch.where(c["tables"] >= 0, c["tables"] + (pages - small), -1).cuda()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    bounds = torch.zeros(pages, 8, 8, 2, 128, dtype=torch.bfloat16, device="cuda")
+    ops.paged_key_bounds_(bounds, big["kc"], moved, i32([0, 0]), c["lens"].cuda(), 1500)
+    assert torch.equal(bounds[pages - small:][c["tables"][0].long()].cpu(), c["bounds"][c["tables"][0].long()].nan_to_num())
+    far = ops.sparse_decode_attention(c["q"].cuda(), big["kc"], big["vc"], bounds, c["lens"].cuda(), moved, c["scale"], 9)
+    near = _call(c, 9)
+    assert all(torch.equal(a, b) for a, b in zip(far, near))
+    group = (c["lens"].cuda(), i32([0, 2]), i32([1]))
+    for variant in (ops.PREFIX_ROWS16, ops.PREFIX_ROWS256):
+        shared = [ops.shared_prefix_decode_attention(c["q"].cuda()[:1].expand(2, 16, 128), k, v, group[0], t, *group[1:],
+                                                     c["scale"], variant=variant)
+                  for k, v, t in ((big["kc"], big["vc"], moved), (c["kc"].cuda(), c["vc"].cuda(), c["tables"].cuda()))]
+        assert torch.equal(*shared)
+    del big, bounds
+    torch.cuda.empty_cache()
+
+
 def test_reports(monkeypatch):
     monkeypatch.setenv("NANOINFER_B200_VALIDATE", "1")
     c = _case(60, 16, 8, 128, 16, 16, [200, 100], poison=False)
