@@ -172,7 +172,7 @@ fork_plan_kernel(const ForkParams p) {
     if (c >= 0 && c < p.rows && __ldg(p.parents + i) != -1) atomicMin(p.winner + c, static_cast<int>(i));
   }
   __syncthreads();
-  int needed = 0;  // forks before this round's that need a page
+  int needed = 0;  // forks of earlier passes that need a page
   for (int64_t i0 = 0; i0 < p.n; i0 += kPlanThreads) {
     const int64_t i = i0 + tid;
     bool ok = false, part = false;
