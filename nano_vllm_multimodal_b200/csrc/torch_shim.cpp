@@ -656,11 +656,12 @@ PageView page_view(const Tensor& cache, int64_t block_dim, const char* what) {
     page *= cache.size(d);
   }
   TORCH_CHECK(v.blocks <= 1 || cache.stride(bd) == page, what, ": the blocks must lie one behind the other");
-  int64_t next = 0;  // the stride that the next outer dim must have
+  int64_t next = -1;  // the stride that the next outer dim must have; any for the innermost, but 0 is none
   for (int64_t d = bd - 1; d >= 0; --d) {
     if (cache.size(d) == 1) continue;
-    TORCH_CHECK(next == 0 || cache.stride(d) == next, what, ": the dims before the blocks must have one stride");
-    if (next == 0) v.plane_stride = cache.stride(d) * es;
+    TORCH_CHECK((next < 0 || cache.stride(d) == next) && (cache.stride(d) > 0 || cache.numel() == 0), what,
+                ": the dims before the blocks must have one stride");
+    if (next < 0) v.plane_stride = cache.stride(d) * es;
     next = cache.stride(d) * cache.size(d);
     v.planes *= cache.size(d);
   }
