@@ -758,8 +758,10 @@ template <typename T, int D, int MODE>
 int launch_combine_partials(const nib_decode_attention_args& a, const MmaDecodeParams& p, cudaStream_t st) {
   static_assert(kCombineBatch * kCombineWarps <= 32, "a batch's weights lie in one warp");
   const int64_t rows = a.batch * a.num_heads;
-  // one warp a row once that gives every SM 16 warps
-  if (rows >= 16LL * sm_count()) {
+  // one warp a row once that gives every SM 16 warps; it stores pairs, for which `out` has to be 4-byte
+  // aligned with even strides (the other form stores single elements)
+  const bool pairs = reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.out_batch_stride % 2 == 0 && a.out_head_stride % 2 == 0;
+  if (pairs && rows >= 16LL * sm_count()) {
     const unsigned grid = static_cast<unsigned>((rows + kCombineWarps - 1) / kCombineWarps);
     launch_k_after(combine_partials_kernel<T, D, MODE, 1>, grid, kCombineWarps * 32, 0, st, p);
   } else {
