@@ -148,7 +148,8 @@ NIB_API int nib_visual_merge(int dtype, const void* token_embeddings, int64_t to
  * fp32, output rounded once. A context length outside [0, max_blocks_per_seq *
  * block_size] sets NIB_DEV_BAD_INDEX and is clamped; a block id outside
  * [0, num_blocks) sets NIB_DEV_BAD_BLOCK and its token is left out. An empty
- * context gives zeros. max_context_len (host upper bound, 0 = from the table
+ * context gives zeros, so does a row whose scores are all -inf; a row that meets a
+ * NaN score or one of +inf is NaN. max_context_len (host upper bound, 0 = from the table
  * width) picks how many CTAs split a context; the partials then need
  * nib_decode_attention_workspace_bytes() bytes of device workspace.
  * Replaces: flash_attn_with_kvcache(q.unsqueeze(1), k_cache, v_cache,

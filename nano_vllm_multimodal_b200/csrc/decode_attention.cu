@@ -116,7 +116,10 @@ template <int P>
 __device__ __forceinline__ void merge_state(float& m, float& l, f2_t* acc, float mo, float lo,
                                             const f2_t* acco) {
   const float M = fmaxf(m, mo);
-  if (M == -INFINITY) return;  // both empty
+  if (M == -INFINITY) {  // both empty, or of NaN scores alone: the sums are 0 or NaN
+    l += lo;
+    return;
+  }
   const float a = ex2f(m - M), b = ex2f(mo - M);
   l = l * a + lo * b;
   const f2_t a2 = f2(a, a), b2 = f2(b, b);
@@ -275,7 +278,11 @@ decode_attention_kernel(const DecodeParams p) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (ok[u]) mx = fmaxf(mx, s[u][j]);
-        if (mx == -INFINITY) continue;  // nothing seen yet
+        if (mx == -INFINITY) {  // nothing seen yet but scores of -inf and NaN, of the weights 0 and NaN
+#pragma unroll
+          for (int u = 0; u < U; ++u) l[j] += ok[u] ? ex2f(s[u][j]) : 0.f;
+          continue;
+        }
         const float r = ex2f(m[j] - mx);
         l[j] *= r;
         const f2_t r2 = f2(r, r);
@@ -346,11 +353,12 @@ decode_attention_kernel(const DecodeParams p) {
         L += r[D + 1] * f;
         A += r[d] * f;
       }
+    } else {
+      for (int t = 0; t < p.token_groups; ++t) L += red[((hgi * p.token_groups + t) * HPW + j) * SW + D + 1];  // 0 or NaN
     }
     const int h = kvh * p.group + hl;
     if (p.splits == 1) {
-      const float o = L > 0.f ? A / L : 0.f;
-      static_cast<T*>(p.out)[b * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(o);
+      static_cast<T*>(p.out)[b * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(attention_row(A, L));
     } else {
       float* ws = p.ws + ((b * p.num_heads + h) * p.splits + split) * SW;
       ws[d] = A;
@@ -398,6 +406,9 @@ decode_combine_kernel(const DecodeParams p) {
           A += o[s] * f;
         }
       }
+    } else {
+#pragma unroll
+      for (int s = 0; s < kCombineUnrolled; ++s) L += l[s];  // 0, or the NaN of NaN scores
     }
   } else {
     for (int s = 0; s < p.splits; ++s) M = fmaxf(M, ws[s * SW + D]);
@@ -407,9 +418,11 @@ decode_combine_kernel(const DecodeParams p) {
         L += ws[s * SW + D + 1] * f;
         A += ws[s * SW + d] * f;
       }
+    } else {
+      for (int s = 0; s < p.splits; ++s) L += ws[s * SW + D + 1];
     }
   }
-  static_cast<T*>(p.out)[b * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : 0.f);
+  static_cast<T*>(p.out)[b * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(attention_row(A, L));
 }
 
 // CTA shape and split count for a launch

@@ -283,9 +283,9 @@ __device__ __forceinline__ void load_q_frags(uint32_t (&qa)[D / 16][4], const T*
 
 // One 16-token tile of a stage (K at kt, V at kt + tile bytes) into the online
 // softmax state of rows r0 (a) and r0 + 8 (b): S = Q K^T, scores of tokens
-// outside [lo, hi) (tile-relative) masked, then O += P V. KEEP_NAN: a row whose scores are all NaN so
-// far keeps a NaN in its sum (and, below, in the result); without, it counts as empty.
-template <typename T, int D, bool KEEP_NAN>
+// outside [lo, hi) (tile-relative) masked, then O += P V. A row whose scores are all NaN so far keeps
+// a NaN in its sum (and, below, in the result): only a row of masked scores counts as empty.
+template <typename T, int D>
 __device__ __forceinline__ void mma_tile(const uint32_t (&qa)[D / 16][4], uint32_t kt, int lo, int hi, float qscale,
                                          float (&o)[D / 8][4], float& m_a, float& m_b, float& l_a, float& l_b,
                                          int lane) {
@@ -327,8 +327,9 @@ __device__ __forceinline__ void mma_tile(const uint32_t (&qa)[D / 16][4], uint32
     mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, off));
   }
   const float na = fmaxf(m_a, mx_a), nb = fmaxf(m_b, mx_b);
-  const float ra = na == -INFINITY ? 1.f : ex2_fast(m_a - na);
-  const float rb = nb == -INFINITY ? 1.f : ex2_fast(m_b - nb);
+  // nothing but masked (-inf) and NaN scores so far: less 0, so that these become 0 and NaN
+  const float sa = na == -INFINITY ? 0.f : na, sb = nb == -INFINITY ? 0.f : nb;
+  const float ra = ex2_fast(m_a - sa), rb = ex2_fast(m_b - sb);
   m_a = na;
   m_b = nb;
   float pa[2][2], pb[2][2];
@@ -336,9 +337,8 @@ __device__ __forceinline__ void mma_tile(const uint32_t (&qa)[D / 16][4], uint32
   for (int nt = 0; nt < 2; ++nt) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      pa[nt][c] = na == -INFINITY ? (KEEP_NAN && s[nt][c] != s[nt][c] ? s[nt][c] : 0.f) : ex2_fast(s[nt][c] - na);
-      pb[nt][c] = nb == -INFINITY ? (KEEP_NAN && s[nt][c + 2] != s[nt][c + 2] ? s[nt][c + 2] : 0.f)
-                                  : ex2_fast(s[nt][c + 2] - nb);
+      pa[nt][c] = ex2_fast(s[nt][c] - sa);
+      pb[nt][c] = ex2_fast(s[nt][c + 2] - sb);
     }
   }
   l_a = l_a * ra + (pa[0][0] + pa[0][1]) + (pa[1][0] + pa[1][1]);
@@ -576,7 +576,7 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     const int lo = from > t0 ? static_cast<int>(from - t0) : 0;
     const int hi = to - t0 < kMmaTile ? static_cast<int>(to - t0) : kMmaTile;
     if (lo > 0 || hi < kMmaTile) zero_rows<D>(dsm + (kt - base_all), lo, hi, lane);
-    mma_tile<T, D, MODE != kDecodeFull>(qa, kt, lo, hi, p.qscale, o, m_a, m_b, l_a, l_b, lane);
+    mma_tile<T, D>(qa, kt, lo, hi, p.qscale, o, m_a, m_b, l_a, l_b, lane);
     __syncwarp();  // every lane has read the stage before it is refilled
   }
 
@@ -630,13 +630,12 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
         L += rr[D + 1] * f;
         A += rr[d] * f;
       }
-    } else if (MODE != kDecodeFull) {
+    } else {
 #pragma unroll
       for (int ww = 0; ww < kMmaWarps; ++ww) L += red[(ww * 16 + r) * SW + D + 1];  // 0, or the NaN of NaN scores
     }
     if (p.ws == nullptr) {
-      const float none = MODE != kDecodeFull && L != L ? L : 0.f;
-      static_cast<T*>(p.out)[rb * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(L > 0.f ? A / L : none);
+      static_cast<T*>(p.out)[rb * p.o_bs + h * p.o_hs + d] = Elem<T>::from_f(attention_row(A, L));
     } else if constexpr (MODE == kDecodeFull) {
       float* ws = p.ws + ((rb * p.num_heads + h) * p.splits + split) * SW;
       ws[d] = A;

@@ -277,6 +277,10 @@ __device__ __forceinline__ float sumsq_tree(const float* v) {
 // same two roundings as `1.0f / sqrtf(x)` without fast math).
 __device__ __forceinline__ float inv_sqrt_rn(float x) { return __frcp_rn(__fsqrt_rn(x)); }
 
+// An element of an attention row from its weighted sum A and the sum L of its weights: zero for a
+// row without tokens (L = 0), NaN for one that met a NaN score (L = NaN).
+__device__ __forceinline__ float attention_row(float A, float L) { return L > 0.f ? A / L : L; }
+
 __device__ __forceinline__ void flag(unsigned int* status, unsigned int bit) {
   if (status != nullptr) atomicOr(status, bit);
 }
