@@ -115,7 +115,8 @@ __device__ __forceinline__ int64_t shared_prefix_of(const MmaDecodeParams& p, in
 }
 
 // Row tile `tile` (tile_rows rows each, a group's last one ragged) of the groups in order:
-// its group's requests and its place among the group's tiles. By a whole warp.
+// its group's requests and its place among the group's tiles. By a whole warp. Tile 0 looks every group
+// over and reports what is wrong, whether or not it has rows.
 struct RowTile {
   int64_t first, end;  // the group's requests
   int64_t row0;        // the tile's first row: row = (request - first) * heads per kv head + head
@@ -133,8 +134,8 @@ __device__ __forceinline__ RowTile find_row_tile(const MmaDecodeParams& p, int64
     if (g < p.num_groups) {
       lo = __ldg(p.group_offsets + g);
       hi = __ldg(p.group_offsets + g + 1);
-      const bool bad = lo < 0 || hi < lo || hi > p.batch;
-      if (bad && tile == 0) flag(p.status, NIB_DEV_BAD_INDEX);
+      const int shared = tile == 0 ? __ldg(p.prefix_lens + g) : 0;
+      if (tile == 0 && (lo < 0 || hi < lo || hi > p.batch || shared < 0)) flag(p.status, NIB_DEV_BAD_INDEX);
       lo = lo < 0 ? 0 : lo;
       hi = hi > p.batch ? p.batch : hi;
       if (hi < lo) hi = lo;
@@ -147,19 +148,18 @@ __device__ __forceinline__ RowTile find_row_tile(const MmaDecodeParams& p, int64
       if (lane >= off) upto += v;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, tile < base + upto);
-    if (hit) {
+    if (hit && found_g < 0) {
       const int src = __ffs(hit) - 1;
       r.first = __shfl_sync(0xffffffffu, lo, src);
       r.end = __shfl_sync(0xffffffffu, hi, src);
       r.row0 = (tile - base - __shfl_sync(0xffffffffu, upto - mine, src)) * tile_rows;
       found_g = g0 + src;
-      break;
+      if (tile > 0) break;
     }
     base += __shfl_sync(0xffffffffu, upto, 31);
   }
   if (found_g < 0) return r;
   const int64_t pre = __ldg(p.prefix_lens + found_g);
-  if (pre < 0 && r.row0 == 0 && lane == 0) flag(p.status, NIB_DEV_BAD_INDEX);
   if (pre <= 0) return r;
   for (int64_t b0 = r.first; b0 < r.end; b0 += 32) {
     const bool holds = b0 + lane < r.end && clamped_len(p, b0 + lane, false) >= pre;
