@@ -223,7 +223,8 @@ NIB_API int nib_shared_prefix_decode_attention(const nib_shared_prefix_args* arg
  * before context_lens[b]. bounds is [num_blocks, num_kv_heads, block_size / chunk, 2, head_dim]
  * of the cache's dtype, the last three dims contiguous; other chunks keep their bytes. A NaN
  * key gives NaN bounds. max_new_tokens (host): the most tokens that a request has between
- * start_lens and context_lens; more set NIB_DEV_BAD_INDEX and are left out from the chunk after.
+ * start_lens and context_lens (0: none has any); more set NIB_DEV_BAD_INDEX, and chunks behind
+ * those that so many tokens can lie in keep their bytes.
  * Two requests may name the same block where their tokens in it are the same.
  * No counterpart in the reference. */
 NIB_API int nib_paged_key_bounds(int dtype, const void* key_cache, int64_t cache_block_stride,

@@ -21,7 +21,8 @@ struct BoundsParams {
   const void* kc;
   int64_t c_bs, c_ss, c_hs;
   int64_t num_blocks;
-  int block_size, chunk, nkv, max_windows;
+  int block_size, chunk, nkv;
+  int64_t max_new;
   const int32_t* tables;
   int64_t table_stride, cap;
   const int32_t* starts;
@@ -64,7 +65,7 @@ key_bounds_kernel(const BoundsParams p) {
   }
   if (start >= len) return;
   const int64_t c = start / p.chunk + blockIdx.x;
-  if (blockIdx.x == 0 && threadIdx.x == 0 && (len - 1) / p.chunk - start / p.chunk >= p.max_windows)
+  if (blockIdx.x == 0 && threadIdx.x == 0 && len - start > p.max_new)
     flag(p.status, NIB_DEV_BAD_INDEX);  // more new tokens than the caller said
   const int64_t t0 = c * p.chunk;
   if (t0 >= len) return;
@@ -717,7 +718,7 @@ extern "C" int nib_paged_key_bounds(int dtype, const void* key_cache, int64_t ca
   NIB_REQUIRE(chunk >= 1 && block_size % chunk == 0, "paged_key_bounds: chunk must divide the block size");
   NIB_SUPPORT(dtype == NIB_BF16 || dtype == NIB_F16, "paged_key_bounds: dtype must be bf16 or f16");
   NIB_SUPPORT(head_dim == 64 || head_dim == 128, "paged_key_bounds: head_dim must be 64 or 128");
-  if (batch == 0 || max_new_tokens == 0 || max_blocks_per_seq == 0) return NIB_OK;
+  if (batch == 0 || max_blocks_per_seq == 0) return NIB_OK;
   NIB_REQUIRE(key_cache && block_tables && start_lens && context_lens && bounds, "paged_key_bounds: null pointer");
   NIB_REQUIRE(block_size < (int64_t{1} << 31) && max_blocks_per_seq * block_size < (int64_t{1} << 31),
               "paged_key_bounds: block table covers too many tokens (2^31 - 4096)");
@@ -743,9 +744,12 @@ extern "C" int nib_paged_key_bounds(int dtype, const void* key_cache, int64_t ca
   p.b_bs = bounds_block_stride;
   p.b_hs = bounds_head_stride;
   p.status = status;
-  const int64_t most = max_new_tokens < p.cap ? max_new_tokens : p.cap;
-  p.max_windows = static_cast<int>((most - 1) / chunk + 2);  // the first new token may sit anywhere in its chunk
-  const dim3 grid(static_cast<unsigned>(p.max_windows), static_cast<unsigned>(batch));
+  p.max_new = max_new_tokens;
+  // the chunks that max_new_tokens can lie in, the first of them anywhere in its chunk; one for none, to
+  // see that there are none
+  const int64_t most = max_new_tokens < p.cap ? max_new_tokens : p.cap, all = p.cap / chunk;
+  const int64_t windows = most == 0 ? 1 : (most - 1) / chunk + 2;
+  const dim3 grid(static_cast<unsigned>(windows < all ? windows : all), static_cast<unsigned>(batch));
   const cudaStream_t st = as_stream(stream);
   if (dtype == NIB_BF16) {
     if (head_dim == 64) launch_k(key_bounds_kernel<__nv_bfloat16, 64>, grid, kBoundsThreads, 0, st, p);

@@ -334,7 +334,8 @@ def paged_key_bounds_(bounds, k_cache, block_tables, start_lens, context_lens, m
     ``bounds`` is ``[blocks, kv_heads, block_size // chunk, 2, head_dim]`` of the cache's dtype: the
     smallest and largest value of each key channel over a chunk's tokens. After a prefill
     ``start_lens`` are the lengths before it, after a decode step ``context_lens - 1``;
-    ``max_new_tokens`` is a host upper bound of their difference."""
+    ``max_new_tokens`` is a host upper bound of their difference (chunks behind those that it allows stay
+    as they are; validation mode raises)."""
     st = _status_for(k_cache)
     _ops().paged_key_bounds_(bounds, k_cache, block_tables, start_lens, context_lens, int(max_new_tokens), st)
     _check_status(st, "paged_key_bounds_")
