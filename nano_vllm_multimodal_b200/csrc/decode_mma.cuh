@@ -114,6 +114,14 @@ __device__ __forceinline__ int64_t shared_prefix_of(const MmaDecodeParams& p, in
   return 0;
 }
 
+// How many of the launch's splits share a request's `own` tokens behind the prefix: 256 tokens each at
+// least. The others write nothing and the merge passes them over.
+constexpr int kOwnTokens = 256;
+__device__ __forceinline__ int own_splits(int64_t own, int splits) {
+  const int64_t n = (own + kOwnTokens - 1) / kOwnTokens;
+  return n < 1 ? 1 : n < splits ? static_cast<int>(n) : splits;
+}
+
 // Row tile `tile` (tile_rows rows each, a group's last one ragged) of the groups in order:
 // its group's requests and its place among the group's tiles. By a whole warp. Tile 0 looks every group
 // over and reports what is wrong, whether or not it has rows.
@@ -394,12 +402,18 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
 
   // kDecodeShared: a 1-D grid; else (rows x kv heads, splits)
   const bool is_prefix = MODE == kDecodeShared && static_cast<int>(blockIdx.x) < p.prefix_ctas;
-  const int splits = is_prefix ? p.prefix_splits : p.splits;
+  int splits = is_prefix ? p.prefix_splits : p.splits;
   int unit = blockIdx.x, split = blockIdx.y;
   if constexpr (MODE == kDecodeShared) {
-    unit -= is_prefix ? 0 : p.prefix_ctas;
-    split = unit % splits;
-    unit /= splits;
+    if (is_prefix) {
+      split = unit % splits;
+      unit /= splits;
+    } else {  // every request's first split before the others, which may have nothing to do
+      const int rows = static_cast<int>(p.batch) * p.num_kv_heads;
+      unit -= p.prefix_ctas;
+      split = unit / rows;
+      unit -= split * rows;
+    }
   }
   const int kvh = unit % p.num_kv_heads;
   int64_t b;          // the request whose table is read
@@ -418,6 +432,11 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
     if constexpr (MODE == kDecodeSuffix || MODE == kDecodeShared) {
       skip = shared_prefix_of(p, b, len, lane);
       len -= skip;
+      splits = own_splits(len, splits);
+      if (split >= splits) {
+        if (MODE == kDecodeSuffix && p.early) pdl_wait();
+        return;
+      }
     }
     if constexpr (MODE == kDecodeSparse) {
       ctx = len;
@@ -654,7 +673,7 @@ decode_attention_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __gr
 
 
 // out[b, h] from the partials of (b, h). MODE kDecodeSuffix: the first slot0 partials are the
-// prefix's, which only a request that shares one has. WPR warps take a row's partials by turns; a
+// prefix's, which only a request that shares one has; behind them as many as its own tokens fill. WPR warps take a row's partials by turns; a
 // warp's first eight outputs are requested together with the maxima and sums, before it is known
 // which of them count: one round trip to memory is most of this kernel's time. (Four warps a row
 // where rows are few, one where they fill the SMs: 4,096 rows of ten partials, 13.2 us with four.)
@@ -678,28 +697,31 @@ combine_partials_kernel(const MmaDecodeParams p) {
   for (int k = 0; k < kCombineBatch; ++k)
     if (part + k * WPR < p.slots) v[k] = ws[static_cast<int64_t>(part + k * WPR) * 32];
   const float2 first = lane < p.slots ? ml[lane] : make_float2(-INFINITY, 0.f);
-  int s0 = 0;
+  int s0 = 0, s1 = p.slots;
   if constexpr (MODE == kDecodeSuffix) {  // and after kDecodeShared
-    if (shared_prefix_of(p, b, clamped_len(p, b, false), lane) == 0) s0 = p.slot0;
+    const int64_t len = clamped_len(p, b, false), shared = shared_prefix_of(p, b, len, lane);
+    if (shared == 0) s0 = p.slot0;
+    s1 = p.slot0 + own_splits(len - shared, p.splits);
   }
-  float M = lane >= s0 ? first.x : -INFINITY;
-  for (int s = 32 + lane; s < p.slots; s += 32)
+  auto counts = [&](int s) { return s >= s0 && s < s1; };
+  float M = counts(lane) ? first.x : -INFINITY;
+  for (int s = 32 + lane; s < s1; s += 32)
     if (s >= s0) M = fmaxf(M, ml[s].x);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
   // a NaN sum (of NaN scores) makes the row NaN
-  bool odd = lane >= s0 && first.y != first.y;
-  for (int s = 32 + lane; s < p.slots; s += 32) odd |= s >= s0 && ml[s].y != ml[s].y;
+  bool odd = counts(lane) && first.y != first.y;
+  for (int s = 32 + lane; s < s1; s += 32) odd |= s >= s0 && ml[s].y != ml[s].y;
   odd = __any_sync(0xffffffffu, odd);
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (M != -INFINITY && !odd) {
     // a split without tokens has no output and the weight 0
-    auto weight = [&](float2 x, int s) { return s >= s0 && x.x != -INFINITY ? ex2_fast(x.x - M) : 0.f; };
+    auto weight = [&](float2 x, int s) { return counts(s) && x.x != -INFINITY ? ex2_fast(x.x - M) : 0.f; };
     const float f = weight(first, lane);
     L = f > 0.f ? first.y * f : 0.f;
-    for (int s = 32 + lane; s < p.slots; s += 32) {
+    for (int s = 32 + lane; s < s1; s += 32) {
       const float2 x = ml[s];
       const float g = weight(x, s);
       if (g > 0.f) L += x.y * g;
@@ -715,9 +737,9 @@ combine_partials_kernel(const MmaDecodeParams p) {
     for (int k = 0; k < kCombineBatch; ++k) {
       const int s = part + k * WPR;  // below 32
       const float g = __shfl_sync(0xffffffffu, f, s);
-      if (s < p.slots && g > 0.f) add(v[k], g);
+      if (s < s1 && g > 0.f) add(v[k], g);
     }
-    for (int s = part + kCombineBatch * WPR; s < p.slots; s += WPR) {
+    for (int s = part + kCombineBatch * WPR; s < s1; s += WPR) {
       const float g = weight(ml[s], s);
       if (g > 0.f) add(ws[static_cast<int64_t>(s) * 32], g);
     }

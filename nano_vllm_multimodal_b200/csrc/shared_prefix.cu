@@ -73,7 +73,16 @@ static SharedPrefixPlan shared_prefix_plan(const nib_shared_prefix_args& s) {
   } else {
     pl.prefix_splits = splits(pl.row_tiles * a.num_kv_heads, max_prefix, 64);
   }
-  pl.suffix_splits = splits(a.batch * a.num_kv_heads, max_len - max_prefix, 256);
+  // What a request has to itself is max_len - max_prefix tokens where its group shares the longest prefix,
+  // but all of them where it is in no group, shorter than its group's prefix, or its group's is short: a
+  // split for each 1,024 of those. How many it uses goes by what it has. us a call, 16/8 heads, with
+  // max_len - max_prefix alone -> so: 32,768 tokens in no group 519 -> 32; four requests of 100 + 16,000
+  // tokens next to four of 20,000 + 50, 274 -> 71; two of 30,000 + 20, whose added splits are empty, 34.0 ->
+  // 33.7. Requests that fill the SMs get one split each, a long one among them too: 32,768 tokens in no
+  // group next to 32 requests of 8,192 + 512, 495 us.
+  const int64_t own = s.num_groups == 0 ? max_len : max_len - max_prefix, by_own = (own + kOwnTokens - 1) / kOwnTokens;
+  const int64_t by_all = (max_len + 1023) / 1024;
+  pl.suffix_splits = splits(a.batch * a.num_kv_heads, (by_own > by_all ? by_own : by_all) * kOwnTokens, kOwnTokens);
   return pl;
 }
 
