@@ -458,7 +458,9 @@ NIB_API int nib_paged_free(const int32_t* block_tables, int64_t table_stride, in
 /* The live blocks (count > 0) move into the first `live` places: the i-th live block behind
  * them to the i-th free place among them, in ascending order. Table entries and counts follow;
  * live (int32 [1]) receives their number, moves (int32 [2, num_blocks / 2]) source and
- * destination of each move, -1 behind the last. The contents of the places that become free
+ * destination of each move, -1 behind the last. Every destination lies before place `live`, every
+ * source from there on: nib_paged_copy_blocks can repeat the moves on what is kept beside the cache,
+ * in pieces of at most 65536 pairs, in any order. The contents of the places that become free
  * stay as they were. workspace: nib_paged_compact_workspace_bytes() bytes. */
 NIB_API int64_t nib_paged_compact_workspace_bytes(int64_t num_blocks);
 NIB_API int nib_paged_compact(void* cache, int64_t planes, int64_t plane_stride_bytes, int64_t num_blocks,

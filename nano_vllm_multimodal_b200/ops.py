@@ -203,8 +203,8 @@ def paged_gather_varlen(cache, block_tables, seq_lens, cu_seqlens, total_tokens:
 def paged_copy_blocks(cache, src_blocks, dst_blocks, block_dim: int = -4) -> None:
     """Copy block ``src_blocks[i]`` to ``dst_blocks[i]`` in every plane (``nib_paged_copy_blocks``).
 
-    A pair with a -1 is skipped. A pair whose destination is another pair's source or
-    destination, or that names no block, is left out (validation mode raises)."""
+    At most 65,536 pairs. A pair with a -1 is skipped. A pair whose destination is another pair's source
+    or destination, or that names no block, is left out (validation mode raises)."""
     st = _status_for(cache)
     _ops().paged_copy_blocks(cache, src_blocks, dst_blocks, int(block_dim), st)
     _check_status(st, "paged_copy_blocks")
@@ -239,7 +239,9 @@ def paged_compact(cache, block_tables, ref_counts, block_dim: int = -4):
     """Move the live blocks to the front -> ``(block_tables, ref_counts, live, moves)``
     (``nib_paged_compact``): the blocks from ``live`` (int32 ``[1]``) on are free afterwards.
     ``moves`` (int32 ``[2, blocks // 2]``: source, destination, -1 behind the last) goes to
-    ``paged_copy_blocks`` for what a program keeps beside the cache."""
+    ``paged_copy_blocks`` for what a program keeps beside the cache; that takes 65,536 pairs a call, and
+    the moves of a cache of more than 131,073 blocks go in pieces of that size
+    (``for src, dst in zip(*(m.split(65536) for m in moves))``), which do not meet."""
     st = _status_for(cache)
     out = _ops().paged_compact(cache, block_tables, ref_counts, int(block_dim), st)
     _check_status(st, "paged_compact")
