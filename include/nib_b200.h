@@ -193,7 +193,8 @@ NIB_API int nib_decode_attention(const nib_decode_attention_args* args, void* st
  * decreasing, within [0, batch]), and the first prefix_lens[g] tokens of all of them hold the
  * same keys and values. Those tokens are read through the table of the group's first request
  * that has as many, once for the group; out[b, h] is what nib_decode_attention gives.
- * A request that is shorter than its group's prefix, or is in no group, is computed by itself.
+ * A request that is shorter than its group's prefix, or is in no group, is computed by itself: by
+ * several CTAs per kv head while requests x kv heads leave SMs free, else by one.
  * A prefix may end inside a block. max_prefix_len and attn.max_context_len (host upper bounds,
  * 0 = from the table width) only choose how the work is split. attn.variant: 0 chooses the prefix's
  * kernel by the rows per group, 1 forces the 16-row kernel, 2 the 256-row one. dtype
@@ -238,10 +239,12 @@ NIB_API int nib_paged_key_bounds(int dtype, const void* key_cache, int64_t cache
 
 /* nib_decode_attention over top_chunks chunks of each context, chosen for each (request, kv
  * head): the first and the last chunk, and those of the others with the largest
- *   score = sum over the kv head's q heads and the channels of max(q lo, q hi),
- * an upper bound of the heads' summed scores of any token in the chunk. Scores are summed in
- * 64 bits; the lower index wins a tie; a NaN or infinite score counts as the largest finite
- * one, a chunk in a block outside [0, num_blocks) as the smallest. Contexts of at most
+ *   score = a . hi + b . lo, a and b the sums of the positive and of the negative parts of the
+ * kv head's q heads: for finite bounds the sum of max(q lo, q hi) over heads and channels, an
+ * upper bound of the heads' summed scores of any token in the chunk. Scores are summed in
+ * 64 bits; the lower index wins a tie; a score of NaN (0 times an infinite bound among them) or
+ * +inf counts as the largest finite one; one of -inf ranks below every finite score, a chunk in a
+ * block outside [0, num_blocks) below that. Contexts of at most
  * top_chunks chunks are attended to whole. selected (int32 [batch, num_kv_heads, top_chunks])
  * receives the chosen chunk indices in ascending order, -1 behind the last.
  * attn.max_context_len (host, 0 = from the table width) bounds the contexts: longer ones are

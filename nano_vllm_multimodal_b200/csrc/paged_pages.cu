@@ -6,8 +6,8 @@
 // p * plane_stride + b * block_bytes. A block table row names a sequence's pages in order, -1
 // behind its last; ref_counts[b] says how many rows name page b, 0: free.
 //
-// Index work is a few kilobytes and one CTA (plan_*); the bytes are moved by a persistent grid
-// in units of (page, plane, 32 KB piece) with 16-byte vectors, eight in flight per thread.
+// Index work is a few kilobytes and one CTA (plan_*); the bytes are moved by a grid of a
+// fixed size in units of (page, plane, 32 KB piece) with 16-byte vectors, eight in flight per thread.
 // Both run behind one another on the stream without a look from the host: how many pages move
 // stays on the device.
 #include "copy_rows.cuh"
@@ -421,7 +421,8 @@ static int page_move(PageMove& m, int& vw, void* cache, int64_t planes, int64_t 
   return NIB_OK;
 }
 
-// a persistent grid: 8 CTAs of 256 threads fill an SM
+// Eight CTAs per SM at most: the movers' 64 to 80 registers (16-byte vectors) let three or four of them run
+// at once, the others follow as SMs become free.
 static unsigned move_grid(const PageMove& m, int vw, int64_t pairs, int64_t at_least) {
   const int64_t piece = static_cast<int64_t>(kMoveThreads) * kMoveVecs * vw;
   int64_t units = pairs * m.planes * ((m.block_bytes + piece - 1) / piece);

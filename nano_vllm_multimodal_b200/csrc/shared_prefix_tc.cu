@@ -12,7 +12,8 @@
 //                  relative, as the operand type of the product wants); its sum is of fp32 values
 //   O += P V       128 x D x 128, P from TMEM, V from shared memory, O in TMEM
 // m is the running maximum, raised only when a tile exceeds it by more than 8 in the exponent (O
-// and the sum are then rescaled): P stays at most 2^8 and the common factor cancels.
+// and the sum are then rescaled): P stays at most 2^8 and the common factor cancels. (A softmax in one pass
+// with a running maximum and sum: Milakov and Gimelshein, Online normalizer calculation for softmax, 2018.)
 //
 // Warps: 0 loads K and V tiles by TMA (5-D tensor maps over the paged cache, 128-byte swizzle,
 // no multicast), 1 and 2 issue a stream's MMAs each, 4-7 and 8-11 are

@@ -44,8 +44,8 @@ constexpr int kBoundsUnroll = 8;
 // One CTA per (window of a request, request): the window's chunk over all kv heads. A thread
 // owns one 16-byte vector of the token row (8 channels of a head) and every slices-th token, eight
 // loads in flight. Bound by HBM for long prefills; three CTAs per SM (16 x 16,384 tokens of 8 x 128
-// 87.5 us, 256 single steps 6.3 us) against four, whose registers spill (85.0 and 7.4), and four with
-// four loads in flight (113.6 and 10.0).
+// 87.5 us, 256 single steps 6.3 us; 80 registers and 16 bytes spilled) against four (64 registers, 28 bytes
+// spilled: 85.0 and 7.4), and four with four loads in flight (113.6 and 10.0).
 template <typename T, int D>
 __global__ void __launch_bounds__(kBoundsThreads, 3)
 key_bounds_kernel(const BoundsParams p) {
@@ -192,7 +192,7 @@ __device__ __forceinline__ uint4 load_bounds(const SelectParams& p, const int32_
 
 constexpr int kScoreWarps = 8;
 constexpr int kScoreUnroll = 8;
-constexpr int kScoreResident = 4;  // CTAs per SM that the registers are sized for
+constexpr int kScoreResident = 4;  // CTAs per SM that the registers are sized for (64; up to 40 bytes spill)
 
 // Scores of a row's chunks in 32 bits, by one of `parts` CTAs. Error: a weight is a sum of at most
 // 16 terms of one sign, a lane adds 8 products with fused operations, five shuffles add the lanes:
